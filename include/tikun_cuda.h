@@ -214,6 +214,64 @@ TK_API int tk_apply_pointwise(const tk_leaf* leaves, size_t n_leaves, int32_t ki
                        void* stream);
 
 /* ---------------------------------------------------------------------- */
+/* gradients between backward and step                                     */
+/* ---------------------------------------------------------------------- */
+
+/* The norm over many gradients, clipping by it, and the sum over
+ * micro-batches.  (Tier 1 of the step above keeps its norm to itself, L2 over
+ * f32 and bf16 leaves, and never changes a gradient.)
+ *
+ * A gradient table describes the tensors once; every call takes it.  out is
+ * where tk_clip_grad_norm and tk_accumulate_grads write: NULL, or the address
+ * and type of g itself, is in place.  All pointers are device memory of the
+ * device that is current in tk_grad_table_create, and calls are made on that
+ * device.  The table holds addresses, not memory: the buffers must outlive its
+ * use.  It is never written after its creation, so threads may share it, and it
+ * may be destroyed while work that was launched with it still runs. */
+typedef struct {
+  const void* g;
+  void* out;         /* may be NULL */
+  uint64_t n;        /* elements, the same in g and out; 0 is allowed */
+  int32_t g_dtype;   /* TK_F32, TK_BF16 or TK_F16 */
+  int32_t out_dtype; /* the same; not read when out is NULL */
+} tk_grad;
+typedef struct tk_grad_table tk_grad_table;
+
+/* TK_ERR_INVALID: a null, host or other device's pointer, an unknown type, an
+ * address that is not a multiple of the element size, an out buffer that
+ * shares memory with any other buffer of the table (its own g in place
+ * excepted). */
+TK_API int tk_grad_table_create(const tk_grad* grads, size_t n, tk_grad_table** out);
+TK_API int tk_grad_table_destroy(tk_grad_table* table);
+
+/* TK_NORM_L2 sqrt(sum x^2), TK_NORM_L1 sum |x|, TK_NORM_MAX max |x|: over all
+ * elements of all tensors, 0 for none.  A NaN element makes each of them NaN.
+ * The sums are formed in a fixed order, so equal inputs give equal bits. */
+enum { TK_NORM_NONE = -1, TK_NORM_L2 = 0, TK_NORM_L1 = 1, TK_NORM_MAX = 2 };
+
+/* The norm, rounded to f32, to *norm_dev; with each_dev, the norm of tensor i
+ * to each_dev[i]; with scale_dev, the clip scale that the step forms of this
+ * norm: max_norm / (norm + 1e-6) if norm > max_norm > 0, else 1 (so also for a
+ * NaN).  All three are device memory and each may be NULL.  Stream-ordered;
+ * does not wait. */
+TK_API int tk_grad_norm(const tk_grad_table* table, int32_t norm, float max_norm, float* norm_dev,
+                        float* each_dev, float* scale_dev, void* stream);
+
+/* out = scale * g, the product formed in f32 and rounded once to out's type,
+ * with the scale of tk_grad_norm; max_norm > 0.  A tensor in place is left as
+ * it is when the scale is 1.  TK_ERR_INVALID if a tensor in place shares
+ * memory with another buffer of the table. */
+TK_API int tk_clip_grad_norm(const tk_grad_table* table, int32_t norm, float max_norm,
+                             float* norm_dev, float* scale_dev, void* stream);
+
+/* out = out + alpha * g (one f32 rounding), or with overwrite out = alpha * g,
+ * for out buffers of TK_F32 that are not in place.  With norm other than
+ * TK_NORM_NONE, the norm of the new out to *norm_dev, formed in the same
+ * pass. */
+TK_API int tk_accumulate_grads(const tk_grad_table* table, float alpha, int32_t overwrite,
+                               int32_t norm, float* norm_dev, void* stream);
+
+/* ---------------------------------------------------------------------- */
 /* Newton-Schulz (Muon)                                                    */
 /* ---------------------------------------------------------------------- */
 

@@ -1,0 +1,443 @@
+"""The gradient operators (tikun_b200.grads) against plain 64-bit forms.
+
+Tolerances, from the roundings that each operator makes (u = 2^-24, half a step
+of f32):
+
+* norm: f32 elements are squared exactly and summed in f64, so that only the
+  last rounding to f32 is left: u.  bf16 and f16 elements are first added by
+  eights in f32, at most five roundings for a group's sum, which is 5 u of an L1
+  norm and half of that of an L2 norm: 6 u with the last one.  The largest
+  magnitude is exact.
+* clipping: given the norm, scale and products are separately rounded f32
+  operations: equal bits.
+* the sum over micro-batches: one f32 rounding of alpha * g + acc: u, and half
+  of the smallest subnormal.  (The 64-bit form rounds once before, which the
+  factor 1.001 covers.)
+"""
+import ctypes
+import math
+import threading
+
+import numpy as np
+import pytest
+import torch
+
+import tikun_b200
+from tikun_b200 import GradTable, _native, accumulate_grads_, clip_grad_norm_, grad_norm
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+IDS = ["f32", "bf16", "f16"]
+NORMS = [2.0, 1.0, math.inf]
+
+
+def tensors(sizes, dtype, seed=0, offsets=(0,), std=None):
+    """Tensors of one buffer each, the first element `offset` elements into it."""
+    gen = torch.Generator().manual_seed(seed)
+    std = std if std is not None else (0.5 if dtype == torch.float16 else 1e-3)
+    out = []
+    for i, n in enumerate(sizes):
+        off = offsets[i % len(offsets)]
+        buf = torch.zeros(off + n + 9, dtype=dtype, device="cuda")
+        buf[off:off + n] = (torch.randn(n, generator=gen) * std).to(dtype)
+        out.append(buf[off:off + n])
+    return out
+
+
+def norm64(ts, p):
+    vals = [t.detach().double().abs().cpu().reshape(-1) for t in ts if t.numel()]
+    if not vals:
+        return 0.0
+    v = torch.cat(vals)
+    if torch.isnan(v).any():
+        return math.nan
+    if p == math.inf:
+        return v.max().item()
+    return math.sqrt((v * v).sum().item()) if p == 2.0 else v.sum().item()
+
+
+def assert_norm(got, want, dtype, p):
+    got = got.item() if isinstance(got, torch.Tensor) else got
+    if math.isnan(want) or math.isinf(want) or p == math.inf:
+        assert got == want or (math.isnan(got) and math.isnan(want)), (got, want)
+        return
+    tol = (1 if dtype == torch.float32 else 6) * U * 1.001
+    assert abs(got - want) <= tol * want + 2.0 ** -150, (got, want, abs(got - want) / max(want, 1e-300))
+
+
+def clip_bits(g, norm, max_norm, dtype):
+    """The clipped gradient from the norm that the call returned, in f32 steps."""
+    norm = np.float32(norm.item())
+    scale = np.float32(1)
+    if norm > np.float32(max_norm):
+        with np.errstate(all="ignore"):
+            scale = np.float32(max_norm) / (norm + np.float32(1e-6))
+    return (g.detach().cpu().float() * torch.tensor(scale)).to(dtype)
+
+
+def same_bits(a, b):
+    a, b = a.detach().cpu(), b.detach().cpu()
+    assert a.dtype == b.dtype and a.shape == b.shape
+    i = torch.int32 if a.dtype == torch.float32 else torch.int16
+    nan = torch.isnan(a) & torch.isnan(b)
+    return bool(((a.view(i) == b.view(i)) | nan).all())
+
+
+SIZES = {
+    "none": [],
+    "empty": [0, 0],
+    "one": [1],
+    "tiny": [1, 0, 7, 8, 9, 0],
+    "unit-edges": list(range(1, 26)),
+    "block-edges": [2047, 2048, 2049, 4097, 256, 65536],
+    "uneven": [1_000_003, 3, 17, 250_000, 1],
+    "many-small": [(i * 37) % 97 for i in range(700)],
+    "three-launches": [(i * 53) % 211 for i in range(2100)],
+    "big-and-small": [5_000_011] + [768] * 40 + [2_000_000],
+}
+
+
+@pytest.mark.parametrize("p", NORMS)
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("sizes", SIZES.values(), ids=SIZES.keys())
+def test_norm(sizes, dtype, p):
+    ts = tensors(sizes, dtype, offsets=(0, 1, 5, 0, 3))
+    got, each = grad_norm(ts, norm_type=p, per_tensor=True)
+    assert got.shape == () and got.dtype == torch.float32 and each.shape == (len(ts),)
+    assert_norm(got, norm64(ts, p), dtype, p)
+    assert_norm(grad_norm(ts, norm_type=p), norm64(ts, p), dtype, p)
+    for t, e in zip(ts, each.tolist()):
+        assert_norm(e, norm64([t], p), dtype, p)
+
+
+@pytest.mark.parametrize("target", ["in-place", "f32", "bf16", "f16"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("sizes", SIZES.values(), ids=SIZES.keys())
+def test_clip(sizes, dtype, target):
+    ts = tensors(sizes, dtype, offsets=(0, 1, 5, 0, 3))
+    before = [t.clone() for t in ts]
+    want = norm64(ts, 2.0)
+    odt = dtype if target == "in-place" else dict(zip(IDS, DTYPES))[target]
+    for max_norm in (want * 0.3 + 1e-9, want * 3 + 1e-9):
+        for t, b in zip(ts, before):
+            t.copy_(b)
+        # out in phase with its gradient, and not
+        outs = None if target == "in-place" else tensors(sizes, odt, seed=1, offsets=(0, 1, 4, 2, 3))
+        norm = clip_grad_norm_(ts, max_norm, out=outs)
+        assert_norm(norm, want, dtype, 2.0)
+        for b, t, o in zip(before, ts, outs or ts):
+            assert same_bits(o, clip_bits(b, norm, max_norm, odt))
+            if outs is not None:
+                assert same_bits(t, b)
+
+
+@pytest.mark.parametrize("p", NORMS)
+def test_clip_by_other_norms(p):
+    ts = tensors([70_001, 33, 8], torch.bfloat16)
+    before = [t.clone() for t in ts]
+    max_norm = 0.5 * norm64(ts, p)
+    norm = clip_grad_norm_(ts, max_norm, norm_type=p)
+    assert_norm(norm, norm64(before, p), torch.bfloat16, p)
+    for b, t in zip(before, ts):
+        assert same_bits(t, clip_bits(b, norm, max_norm, torch.bfloat16))
+
+
+def test_what_lies_around_the_tensors_stays():
+    """Nothing outside the elements is written, at any start and length of a unit."""
+    for dtype in DTYPES:
+        for off in range(9):
+            for n in (1, 6, 8, 9, 17, 4099):
+                buf = torch.full((off + n + 16,), 2.0, dtype=dtype, device="cuda")
+                acc = torch.full((off + n + 16,), 3.0, device="cuda")
+                g = buf[off:off + n]
+                accumulate_grads_([g], [acc[off:off + n]], alpha=0.5)
+                clip_grad_norm_([g], 1e-3)
+                for t, v in ((buf, 2.0), (acc, 3.0)):
+                    assert (t[:off] == v).all() and (t[off + n:] == v).all()
+                assert (acc[off:off + n] == 4.0).all() and (g < 1.0).all()
+
+
+@pytest.mark.parametrize("p", [None] + NORMS)
+@pytest.mark.parametrize("overwrite", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("sizes", SIZES.values(), ids=SIZES.keys())
+def test_accumulate(sizes, dtype, overwrite, p):
+    ts = tensors(sizes, dtype, offsets=(0, 1, 5, 0, 3))
+    acc = tensors(sizes, torch.float32, seed=2, offsets=(0, 1, 4, 2, 3))
+    alpha = 0.3
+    want = [np.float32(alpha).item() * t.double() + (0 if overwrite else a.double())
+            for t, a in zip(ts, acc)]
+    norm = accumulate_grads_(ts, acc, alpha=alpha, overwrite=overwrite, norm_type=p)
+    for a, w in zip(acc, want):
+        err = (a.double() - w).abs()
+        assert (err <= U * 1.001 * w.abs() + 2.0 ** -150).all()
+    if p is None:
+        assert norm is None
+    else:
+        assert_norm(norm, norm64(acc, p), torch.float32, p)
+
+
+def test_types_mixed_in_one_call():
+    ts = [t for d in DTYPES for t in tensors([1000, 3, 70_000], d, std=0.25)]
+    outs = [torch.empty_like(t, dtype=d) for t, d in zip(ts, DTYPES * 3)]
+    got, each = grad_norm(ts, per_tensor=True)
+    assert_norm(got, norm64(ts, 2.0), torch.bfloat16, 2.0)
+    for t, e in zip(ts, each.tolist()):
+        assert_norm(e, norm64([t], 2.0), t.dtype, 2.0)
+    norm = clip_grad_norm_(ts, 1.0, out=outs)
+    assert same_bits(norm, got)
+    for t, o in zip(ts, outs):
+        assert same_bits(o, clip_bits(t, norm, 1.0, o.dtype))
+
+
+@pytest.mark.parametrize("p", NORMS)
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("value", ["large", "small", "subnormal", "mixed", "zeros", "inf", "-inf", "nan"])
+def test_values_at_the_ends_of_the_range(value, dtype, p):
+    info = torch.finfo(dtype)
+    n = 5003
+    x = torch.zeros(n, dtype=torch.float64)
+    if value == "large":  # squares, and sums of f32, overflow f32
+        x[:] = info.max
+    elif value == "small":  # squares underflow f32
+        x[:] = info.tiny * 3
+    elif value == "subnormal":
+        x[:] = info.smallest_normal * info.eps * 5
+    elif value == "mixed":  # eights of both kinds, and some whose squares underflow beside ones
+        x[:] = 1e-30
+        x[5::64] = -info.max / 4
+        x[2::40] = 1.0
+    elif value != "zeros":
+        x[:] = 0.5
+        x[n // 2] = float(value)
+    t = x.to(dtype).cuda()
+    ts = [t[:2000], t[2000:2001], t[2001:]]
+    got, each = grad_norm(ts, norm_type=p, per_tensor=True)
+    assert_norm(got, f32_range(norm64(ts, p)), dtype, p)
+    for s, e in zip(ts, each.tolist()):
+        assert_norm(e, f32_range(norm64([s], p)), dtype, p)
+
+
+def f32_range(v):
+    """A norm above f32's range is infinity."""
+    return math.inf if v >= 2.0 ** 128 else v
+
+
+@pytest.mark.parametrize("value", ["inf", "nan"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_clip_of_non_finite_gradients(dtype, value):
+    """A NaN norm leaves the gradients, an infinite one scales them by 0."""
+    ts = tensors([1000, 50], dtype)
+    ts[1][7] = float(value)
+    before = [t.clone() for t in ts]
+    with pytest.raises(RuntimeError, match="norm of order 2.0 is " + value):
+        clip_grad_norm_(ts, 1.0, error_if_nonfinite=True)
+    assert all(same_bits(t, b) for t, b in zip(ts, before))
+    with pytest.raises(RuntimeError, match="is " + value):
+        grad_norm(ts, error_if_nonfinite=True)
+    norm = clip_grad_norm_(ts, 1.0)
+    for b, t in zip(before, ts):
+        assert same_bits(t, clip_bits(b, norm, 1.0, dtype))
+    if value == "inf":
+        assert (ts[0] == 0).all() and math.isnan(ts[1][7].item())
+
+
+def test_equal_inputs_give_equal_bits():
+    for dtype in DTYPES:
+        ts = tensors([3_000_001, 77, 1_000_000], dtype)
+        a = [grad_norm(ts, norm_type=p, per_tensor=True) for p in NORMS]
+        b = [grad_norm(ts, norm_type=p, per_tensor=True) for p in NORMS]
+        for (x, xe), (y, ye) in zip(a, b):
+            assert same_bits(x, y) and same_bits(xe, ye)
+
+
+def test_dense_views_in_other_orders():
+    w = torch.randn(40, 70, device="cuda")
+    g = w.t()  # a transposed weight's gradient
+    assert not g.is_contiguous()
+    assert_norm(grad_norm([g]), norm64([w], 2.0), torch.float32, 2.0)
+    out = torch.empty_like(g, dtype=torch.bfloat16)  # keeps the strides
+    assert out.stride() == g.stride()
+    norm = clip_grad_norm_([g], 1.0, out=[out])
+    assert same_bits(out, clip_bits(g, norm, 1.0, torch.bfloat16))
+    with pytest.raises(ValueError, match="strides"):
+        clip_grad_norm_([g], 1.0, out=[torch.empty(70, 40, device="cuda")])
+    for bad in (w[:, ::2], w[:, 1:], torch.zeros(3, 1, device="cuda").expand(3, 4)):
+        with pytest.raises(ValueError, match="one stretch of memory"):
+            grad_norm([bad])
+
+
+def test_refusals_with_device_tensors():
+    a = torch.zeros(64, device="cuda")
+    with pytest.raises(TypeError, match="float64"):
+        grad_norm([a.double()])
+    with pytest.raises(ValueError, match="1 out tensors for 2 gradients"):
+        clip_grad_norm_([a, a.clone()], 1.0, out=[a.clone()])
+    with pytest.raises(ValueError, match="out 0 has shape"):
+        clip_grad_norm_([a], 1.0, out=[torch.zeros(63, device="cuda")])
+    # twice the same tensor: counted twice by the norm, refused by the clip
+    a += 1.0
+    assert grad_norm([a, a]).item() == np.float32(math.sqrt(128.0))
+    with pytest.raises(ValueError, match="shares memory"):
+        clip_grad_norm_([a, a], 1.0)
+    with pytest.raises(ValueError, match="shares memory"):
+        clip_grad_norm_([a, a[8:9]], 1.0)
+    with pytest.raises(ValueError, match="overlap"):
+        clip_grad_norm_([a[:32]], 1.0, out=[a[16:48]])
+    assert (a == 1.0).all()
+    # sums go into f32 buffers of their own
+    for acc in (a, torch.zeros(64, device="cuda", dtype=torch.bfloat16)):
+        with pytest.raises(ValueError, match="f32 out buffers of their own"):
+            accumulate_grads_([a], [acc])
+    with pytest.raises(ValueError, match="f32 out buffers of their own"):
+        accumulate_grads_(GradTable([a]))
+    with pytest.raises(ValueError, match="has its out tensors"):
+        clip_grad_norm_(GradTable([a]), 1.0, out=[a])
+    pinned = torch.zeros(8).pin_memory()
+    arr = (_native.TkGrad * 1)(_native.TkGrad(pinned.data_ptr(), 0, 8, 0, 0))
+    h = ctypes.c_void_p()
+    with pytest.raises(ValueError, match="not device memory"):
+        _native.check(_native.lib().tk_grad_table_create(arr, 1, ctypes.byref(h)))
+
+
+def test_parameters_stand_for_their_gradients():
+    lin = torch.nn.Linear(33, 17, device="cuda")
+    frozen = torch.nn.Parameter(torch.zeros(5, device="cuda"))
+    lin(torch.randn(8, 33, device="cuda")).square().sum().backward()
+    want = norm64([p.grad for p in lin.parameters()], 2.0)
+    table = GradTable({"a": list(lin.parameters()), "b": frozen, "c": None})
+    assert len(table) == 2
+    assert_norm(grad_norm(table), want, torch.float32, 2.0)
+    assert_norm(grad_norm(lin.parameters()), want, torch.float32, 2.0)
+    ref = [p.grad.clone() for p in lin.parameters()]
+    norm = clip_grad_norm_(lin.parameters(), want / 2)
+    for p, b in zip(lin.parameters(), ref):
+        assert same_bits(p.grad, clip_bits(b, norm, want / 2, torch.float32))
+    lin.zero_grad(set_to_none=True)
+    with pytest.raises(RuntimeError, match="build the table anew"):
+        grad_norm(table)
+    assert grad_norm(lin.parameters()).item() == 0.0
+
+
+def test_micro_batches_norm_clip_and_step_together():
+    """Sum, norm, clip and an AdamW step that does not clip give the bits of the
+    fused clipped step on the same sums; the clipped bf16 gradients, too, of
+    the torch form of the whole path."""
+    sizes = [4099, 768, 1, 250_000]
+    parts = [tensors(sizes, torch.bfloat16, seed=s) for s in range(3)]
+    acc = [torch.empty(n, device="cuda") for n in sizes]
+    for k, gs in enumerate(parts):
+        norm = accumulate_grads_(gs, acc, alpha=1 / 3, overwrite=k == 0,
+                                 norm_type=2.0 if k == 2 else None)
+    max_norm = 0.25 * norm.item()
+    params = [torch.randn(n, device="cuda") * 0.02 for n in sizes]
+    a = [torch.nn.Parameter(p.clone()) for p in params]
+    b = [torch.nn.Parameter(p.clone()) for p in params]
+    opt_a = tikun_b200.AdamW(a, max_norm=max_norm)
+    opt_a.step([t.clone() for t in acc])
+    low = [torch.empty_like(t, dtype=torch.bfloat16) for t in acc]
+    clip_grad_norm_(acc, max_norm, out=low)
+    again = clip_grad_norm_(acc, max_norm)
+    assert same_bits(again, norm)
+    opt_b = tikun_b200.AdamW(b)
+    opt_b.step(acc)
+    for x, y, t, l in zip(a, b, acc, low):
+        assert same_bits(x, y)
+        assert same_bits(l, t.to(torch.bfloat16))
+    plain = [sum(np.float32(1 / 3).item() * gs[i].double() for gs in parts) for i in range(len(sizes))]
+    n64 = math.sqrt(sum((x * x).sum().item() for x in plain))
+    for x, t in zip(plain, acc):
+        want = x * (max_norm / (n64 + 1e-6))
+        # three sums, norm, scale (two roundings) and product
+        assert ((t.double() - want).abs() <= 8 * U * x.abs().max() + 2.0 ** -149).all()
+
+
+def test_captured_calls_and_graphs_side_by_side():
+    """Two captured graphs on two streams, replayed at once on new contents,
+    beside eager calls on a third."""
+    sizes = [100_003, 768, 5]
+    side = [torch.cuda.Stream() for _ in range(2)]
+    graphs, state = [], []
+    for k in range(2):
+        ts = tensors(sizes, torch.bfloat16, seed=k)
+        outs = [torch.empty_like(t, dtype=torch.float32) for t in ts]
+        table = GradTable(ts, out=outs)
+        clip_grad_norm_(table, 0.01)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side[k]):
+            norm = clip_grad_norm_(table, 0.01)
+            total, each = grad_norm(ts, per_tensor=True)
+        graphs.append(g)
+        state.append((ts, outs, norm, total, each))
+    eager = tensors(sizes, torch.float32, seed=9)
+    for round_ in range(3):
+        for k in range(2):
+            for t, n in zip(state[k][0], tensors(sizes, torch.bfloat16, seed=10 * round_ + k)):
+                t.copy_(n)
+        torch.cuda.synchronize()
+        for _ in range(4):
+            for k in range(2):
+                with torch.cuda.stream(side[k]):
+                    graphs[k].replay()
+            e = grad_norm(eager)
+        torch.cuda.synchronize()
+        assert_norm(e, norm64(eager, 2.0), torch.float32, 2.0)
+        for ts, outs, norm, total, each in state:
+            want = norm64(ts, 2.0)
+            assert_norm(norm, want, torch.bfloat16, 2.0)
+            assert same_bits(norm, total)
+            for t, o, x in zip(ts, outs, each.tolist()):
+                assert same_bits(o, clip_bits(t, norm, 0.01, torch.float32))
+                assert_norm(x, norm64([t], 2.0), torch.bfloat16, 2.0)
+
+
+def test_streams_and_threads():
+    """Calls on a side stream order after that stream's work; threads share a table."""
+    n = 3_000_000
+    s = torch.cuda.Stream()
+    g = torch.zeros(n, device="cuda")
+    table = GradTable([g])
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        for _ in range(20):
+            g.add_(1.0)
+        norm = grad_norm(table, norm_type=1.0)
+        g.zero_()
+    s.synchronize()
+    assert norm.item() == 20.0 * n
+    g.fill_(2.0)
+    torch.cuda.synchronize()
+    got = [[] for _ in range(4)]
+
+    def work(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(50):
+                got[k].append(grad_norm(table, norm_type=[2.0, 1.0, math.inf, 2.0][k]))
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    want = [np.float32(2.0 * math.sqrt(n)), 2.0 * n, 2.0, np.float32(2.0 * math.sqrt(n))]
+    for k in range(4):
+        assert len(got[k]) == 50 and all(x.item() == want[k] for x in got[k])
+
+
+def test_more_than_two_to_the_32_elements():
+    """Element offsets and byte offsets past 32 bits."""
+    n = 2 ** 32 + 4099
+    g = torch.ones(n, dtype=torch.bfloat16, device="cuda")
+    g[-1] = 3.0
+    total, each = grad_norm([g[:5], g[5:]], norm_type=1.0, per_tensor=True)
+    assert total.item() == np.float32(n + 2) and each[0].item() == 5.0
+    assert grad_norm([g], norm_type=math.inf).item() == 3.0
+    norm = clip_grad_norm_([g], 0.5 * n, norm_type=1.0)
+    assert norm.item() == np.float32(n + 2)
+    assert same_bits(g[-5000:], clip_bits(torch.cat([torch.ones(4999), torch.tensor([3.0])]).bfloat16(),
+                                          norm, 0.5 * n, torch.bfloat16))
+    assert same_bits(g[2 ** 31 - 8:2 ** 31 + 8], g[:16]) and same_bits(g[2 ** 32 - 8:2 ** 32 + 8], g[:16])

@@ -4,6 +4,9 @@ Front-ends with the reference's names and arguments (python/tikun/__init__.py):
 ``Optimizer`` (UniversalOptimizer), ``AdamW``, ``Lion``, ``SGD``, ``Muon`` and
 ``MuonND`` (MultiDimensionalMuon).  The native
 entry points of the reference's ``_tikun`` module are in ``tikun_b200._native``.
+
+Beside them, for the gradients between backward and step (``tikun_b200.grads``):
+``grad_norm``, ``clip_grad_norm_``, ``accumulate_grads_`` and ``GradTable``.
 """
 from .universal import UniversalOptimizer as Optimizer
 from .universal import UniversalOptimizer
@@ -35,13 +38,18 @@ def SGD(params, lr=1e-2, momentum=0.9, weight_decay=0.0, max_norm=0.0, in_backwa
 
 
 def __getattr__(name):
-    # Muon subclasses torch.optim.Optimizer: import torch only when it is asked for
+    # these import torch: only when one is asked for
     if name in ("Muon", "zeropower_via_newtonschulz5"):
         from . import muon
 
         return getattr(muon, name)
+    if name in ("GradTable", "grad_norm", "clip_grad_norm_", "accumulate_grads_"):
+        from . import grads
+
+        return getattr(grads, name)
     raise AttributeError(name)
 
 
 __all__ = ["Optimizer", "UniversalOptimizer", "AdamW", "Lion", "SGD", "Muon", "MuonND",
-           "MultiDimensionalMuon", "zeropower_via_newtonschulz5"]
+           "MultiDimensionalMuon", "zeropower_via_newtonschulz5", "GradTable", "grad_norm",
+           "clip_grad_norm_", "accumulate_grads_"]

@@ -29,6 +29,7 @@ TK_F32, TK_BF16, TK_F16 = 0, 1, 2
 TK_ADAMW, TK_LION, TK_SGD, TK_CUSTOM = 0, 1, 2, 3
 TK_ROLE_LOAD, TK_ROLE_COMPUTE, TK_ROLE_STORE = 0, 1, 2
 TK_NS_F16, TK_NS_BF16, TK_NS_F16X3, TK_NS_F16X2 = 0, 1, 2, 3
+TK_NORM_NONE, TK_NORM_L2, TK_NORM_L1, TK_NORM_MAX = -1, 0, 1, 2
 
 
 class TkLeaf(ctypes.Structure):
@@ -67,6 +68,16 @@ class TkMuonHParams(ctypes.Structure):
         ("nesterov", ctypes.c_int32),
         ("ns_steps", ctypes.c_int32),
         ("precision", ctypes.c_int32),
+    ]
+
+
+class TkGrad(ctypes.Structure):
+    _fields_ = [
+        ("g", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("n", ctypes.c_uint64),
+        ("g_dtype", ctypes.c_int32),
+        ("out_dtype", ctypes.c_int32),
     ]
 
 
@@ -166,6 +177,11 @@ _SIGNATURES = {
     "tk_stream_wait_deadline": [_P, _I32, _P],
     "tk_step_buffers_noalloc": [ctypes.POINTER(TkLeaf), _SZ, _I32, ctypes.POINTER(TkHParams),
                                 _U64, _F, ctypes.POINTER(_F), _P],
+    "tk_grad_table_create": [ctypes.POINTER(TkGrad), _SZ, ctypes.POINTER(_P)],
+    "tk_grad_table_destroy": [_P],
+    "tk_grad_norm": [_P, _I32, _F, _P, _P, _P, _P],
+    "tk_clip_grad_norm": [_P, _I32, _F, _P, _P, _P],
+    "tk_accumulate_grads": [_P, _F, _I32, _I32, _P, _P],
     "tk_newton_schulz_2d": [_P, _I64, _I64, _I32, _I32, _I32, _P],
     "tk_newton_schulz_3d": [_P, _I64, _I64, _I64, _I32, _I32, _I32, _P],
     "tk_muon_step": [ctypes.POINTER(TkMuonLeaf), _SZ, ctypes.POINTER(TkMuonHParams), _P],

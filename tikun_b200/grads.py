@@ -1,0 +1,224 @@
+"""Gradients between backward and step, on the B200 engine: the norm over many
+tensors, clipping by it, and the sum over micro-batches.
+
+The optimizers clip by themselves (``max_norm``): they form the global L2 norm
+and fold the scale into their update, so that neither the norm nor a clipped
+gradient ever reaches memory.  The functions here are for programs that need
+those: a norm for the log (of the whole model, or of each tensor), clipped
+gradients for a consumer that does not clip, one norm over the gradients of
+several optimizers, or f32 sums of bf16 or f16 micro-batch gradients.
+
+Gradients are a PyTree (as ``UniversalOptimizer`` takes it) of CUDA tensors of
+one device, f32, bf16 or f16, in any mix and any number.  A ``Parameter``
+stands for its ``.grad``, so ``model.parameters()`` may be given; a parameter
+without a gradient, and ``None``, are left out.  A gradient may be any dense
+view without gaps (a transposed weight's gradient is one).  A program whose
+gradient buffers stand (``arena=True``, or ``zero_grad(set_to_none=False)``)
+builds a ``GradTable`` of them once and gives that in their place: the checks
+and the table's layout are a third to nine tenths of a call's host time.
+
+Every call runs on torch's current stream of the gradients' device and does not
+wait for it (``error_if_nonfinite=True`` does).  A call may be captured into a
+CUDA graph.  No call is seen by autograd.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import _native
+from .universal import flatten_leaves
+
+_NORMS = {2.0: _native.TK_NORM_L2, 1.0: _native.TK_NORM_L1, math.inf: _native.TK_NORM_MAX}
+_DTYPES = {torch.float32: _native.TK_F32, torch.bfloat16: _native.TK_BF16,
+           torch.float16: _native.TK_F16}
+
+
+def _norm_code(norm_type) -> int:
+    code = _NORMS.get(float(norm_type))
+    if code is None:
+        raise ValueError(f"norm_type is 2, 1 or inf, got {norm_type!r}")
+    return code
+
+
+def _dense(t: torch.Tensor) -> bool:
+    """Whether t's elements fill one stretch of memory, in whatever order."""
+    if t.is_contiguous():
+        return True
+    span = 1
+    for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != span:
+            return False
+        span *= size
+    return True
+
+
+def _check(t, what: str) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{what}: expected a torch tensor, got {type(t).__name__}")
+    if t.layout != torch.strided or not t.is_cuda:
+        raise ValueError(f"{what}: expected a dense CUDA tensor, got {t.layout} on {t.device}")
+    if t.dtype not in _DTYPES:
+        raise TypeError(f"{what} is float32, bfloat16 or float16, got {t.dtype}")
+    if t.numel() and not _dense(t):
+        raise ValueError(f"{what}: its elements do not fill one stretch of memory (shape "
+                         f"{tuple(t.shape)}, strides {t.stride()})")
+
+
+class GradTable:
+    """The gradients of one or many calls, checked and laid out once.
+
+    ``out`` (a PyTree of as many CUDA tensors, element i of the size and the
+    strides of gradient i) is where ``clip_grad_norm_`` and
+    ``accumulate_grads_`` write; without it they work in place.  The table keeps
+    the tensors alive and reads and writes the memory they have now.  For
+    parameters it is their ``.grad`` of now: a call raises ``RuntimeError`` once
+    one of them has another (as after ``zero_grad(set_to_none=True)``)."""
+
+    def __init__(self, grads, out=None):
+        self._handle = None
+        self._params = []
+        self.grads = []
+        for leaf in flatten_leaves(grads):
+            if isinstance(leaf, torch.nn.Parameter):
+                if leaf.grad is None:
+                    continue
+                self._params.append((leaf, leaf.grad))
+                leaf = leaf.grad
+            elif leaf is None:
+                continue
+            _check(leaf, f"gradient {len(self.grads)}")
+            self.grads.append(leaf)
+        self.out = None if out is None else flatten_leaves(out)
+        n = len(self.grads)
+        if self.out is not None:
+            if len(self.out) != n:
+                raise ValueError(f"{len(self.out)} out tensors for {n} gradients")
+            for i, (g, o) in enumerate(zip(self.grads, self.out)):
+                _check(o, f"out {i}")
+                if o.numel() != g.numel() or not (
+                        g.is_contiguous() and o.is_contiguous() or o.stride() == g.stride()):
+                    raise ValueError(f"out {i} has shape {tuple(o.shape)} and strides "
+                                     f"{o.stride()}, its gradient {tuple(g.shape)} and "
+                                     f"{g.stride()}")
+        devices = {t.device for t in self.grads + (self.out or [])}
+        if len(devices) > 1:
+            raise ValueError("the tensors of one call are on one device, got "
+                             f"{sorted(map(str, devices))}")
+        self.device = devices.pop() if devices else torch.device("cuda", torch.cuda.current_device())
+        arr = (_native.TkGrad * max(n, 1))()
+        for i, g in enumerate(self.grads):
+            o = self.out[i] if self.out is not None else None
+            arr[i] = _native.TkGrad(g.data_ptr(), 0 if o is None else o.data_ptr(), g.numel(),
+                                    _DTYPES[g.dtype], 0 if o is None else _DTYPES[o.dtype])
+        handle = ctypes.c_void_p()
+        with torch.cuda.device(self.device):
+            _native.check(_native.lib().tk_grad_table_create(arr, n, ctypes.byref(handle)))
+        self._handle = handle
+
+    def __len__(self) -> int:
+        return len(self.grads)
+
+    def __del__(self):
+        if getattr(self, "_handle", None) is not None:
+            _native.lib().tk_grad_table_destroy(self._handle)
+            self._handle = None
+
+    def _standing(self) -> "GradTable":
+        for p, g in self._params:
+            if p.grad is not g:
+                raise RuntimeError("a parameter of this GradTable has another gradient tensor "
+                                   "now: build the table anew")
+        return self
+
+
+def _table(grads, out=None) -> GradTable:
+    if isinstance(grads, GradTable):
+        if out is not None:
+            raise ValueError("a GradTable has its out tensors already")
+        return grads._standing()
+    return GradTable(grads, out)
+
+
+def _finite(norm: torch.Tensor, norm_type) -> None:
+    v = norm.item()
+    if not math.isfinite(v):
+        raise RuntimeError(f"the gradients' norm of order {norm_type} is {v}")
+
+
+def grad_norm(grads, norm_type: float = 2.0, per_tensor: bool = False,
+              error_if_nonfinite: bool = False):
+    """The norm of all gradients' elements as one vector, a 0-dim f32 tensor:
+    sqrt(sum x^2) (2), sum |x| (1) or max |x| (``inf``); 0 without elements,
+    NaN with a NaN among them.  Sums are formed in f64 in a fixed order and
+    rounded once.
+
+    ``per_tensor=True``: (norm, norms), ``norms`` the f32 norms of the
+    gradients, one each."""
+    code = _norm_code(norm_type)
+    t = _table(grads)
+    with torch.cuda.device(t.device):
+        norm = torch.empty((), dtype=torch.float32, device=t.device)
+        each = torch.empty(len(t), dtype=torch.float32, device=t.device) if per_tensor else None
+        _native.check(_native.lib().tk_grad_norm(
+            t._handle, code, 0.0, norm.data_ptr(), each.data_ptr() if len(t) and per_tensor else None,
+            None, torch.cuda.current_stream().cuda_stream))
+    if error_if_nonfinite:
+        _finite(norm, norm_type)
+    return (norm, each) if per_tensor else norm
+
+
+def clip_grad_norm_(grads, max_norm: float, norm_type: float = 2.0, out=None,
+                    error_if_nonfinite: bool = False) -> torch.Tensor:
+    """Scales the gradients by ``max_norm / (norm + 1e-6)`` if their norm (see
+    ``grad_norm``) exceeds ``max_norm``, in place or into ``out``, and returns
+    the norm from before.  Each product is formed in f32 and rounded once to its
+    target's type.  The scale is the one that an optimizer with this
+    ``max_norm`` folds into its update, so clipping f32 gradients here and
+    stepping without ``max_norm`` gives the same bits.
+
+    A norm of NaN leaves the gradients as they are (in place) or copies them
+    (``out``), as the optimizers do; an infinite one makes the scale 0.
+    ``error_if_nonfinite=True`` raises ``RuntimeError`` for both before
+    anything is written, and waits for the norm to know."""
+    code = _norm_code(norm_type)
+    if not max_norm > 0:
+        raise ValueError(f"max_norm is positive, got {max_norm!r}")
+    t = _table(grads, out)
+    with torch.cuda.device(t.device):
+        norm = torch.empty((), dtype=torch.float32, device=t.device)
+        stream = torch.cuda.current_stream().cuda_stream
+        if error_if_nonfinite:
+            _native.check(_native.lib().tk_grad_norm(t._handle, code, 0.0, norm.data_ptr(), None,
+                                                     None, stream))
+            _finite(norm, norm_type)
+        _native.check(_native.lib().tk_clip_grad_norm(t._handle, code, max_norm, norm.data_ptr(),
+                                                      None, stream))
+    return norm
+
+
+def accumulate_grads_(grads, acc=None, alpha: float = 1.0, overwrite: bool = False,
+                      norm_type: float | None = None) -> torch.Tensor | None:
+    """``acc += alpha * grad`` for every gradient, or ``acc = alpha * grad``
+    with ``overwrite`` (the first micro-batch: ``acc`` need not be cleared).
+    ``acc`` (the ``out`` of a ``GradTable``) is f32 whatever the gradients are:
+    sums of micro-batches in bf16 lose the small ones.  ``alpha`` is a host
+    number, such as one over the micro-batches or over a loss scale.
+
+    ``norm_type``: returns the norm of the new ``acc`` (see ``grad_norm``),
+    formed as it is written; otherwise None."""
+    code = _native.TK_NORM_NONE if norm_type is None else _norm_code(norm_type)
+    if not isinstance(grads, GradTable) and acc is None:
+        raise ValueError("accumulate_grads_ needs acc")
+    t = _table(grads, acc)
+    with torch.cuda.device(t.device):
+        norm = torch.empty((), dtype=torch.float32, device=t.device) if norm_type is not None else None
+        _native.check(_native.lib().tk_accumulate_grads(
+            t._handle, alpha, 1 if overwrite else 0, code,
+            norm.data_ptr() if norm is not None else None, torch.cuda.current_stream().cuda_stream))
+    return norm
+
+
+__all__ = ["GradTable", "grad_norm", "clip_grad_norm_", "accumulate_grads_"]
