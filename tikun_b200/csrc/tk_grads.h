@@ -5,67 +5,104 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <memory>
 
 #include "tk_internal.h"
 
 namespace tk {
 namespace gr {
 
-// One tensor.  Its elements stand at positions [phase, phase + n) from `g`,
-// the gradient's address rounded down to a whole unit of kUnit elements, so
-// that unit u (positions kUnit*u .. kUnit*u + 7) is one aligned vector access.
-// `out` is the target's address less the same `phase` elements.
+// Elements are handled in units of kUnit, one vector access each, and the
+// units of a tensor in tiles of 32 KB of gradients, one CTA each.
 constexpr int kUnit = 8;
+template <int G_DTYPE>
+constexpr int kTileUnits = G_DTYPE == TK_F32 ? 1024 : 2048;
+
+// One tensor.  Its elements stand at positions [phase, phase + n) from `g`,
+// the gradient's address rounded down to a whole unit, so that unit u
+// (positions kUnit*u .. kUnit*u + 7) is one aligned access.  `out` is the
+// target's address less the same `phase` elements.  t_begin counts the tiles
+// over the launch.
 struct GradDesc {
   const char* g;
   char* out;
-  uint64_t n;
-  uint64_t u_begin : 44;    // first unit of this tensor in its launch
+  uint64_t n : 44;
   uint64_t phase : 4;
-  uint64_t g_dtype : 4;
   uint64_t out_dtype : 4;
-  uint64_t out_vec : 4;     // out's units are aligned for vector access too
-  uint64_t in_place : 4;    // out is the gradient itself
+  uint64_t out_vec : 4;   // out's units are aligned for vector access too
+  uint64_t in_place : 8;  // out is the gradient itself
+  uint32_t t_begin;
+  uint32_t id;            // its place in the caller's list
 };
 static_assert(sizeof(GradDesc) == 32, "one descriptor is 32 bytes of kernel parameters");
 
-// The tensors of one launch travel in the kernel's parameters, as the leaf
-// tables of the step do.
+// The tensors of one launch, all of one type, travel in the kernel's
+// parameters, as the leaf tables of the step do: the smallest of three tables
+// that holds them, since a launch copies its parameters (host time of a launch
+// with 2, 10 and 31 kB of them: 3, 4 and 6 us).
 constexpr int kMaxGrads = 960;
 template <int CAP>
 struct GradLaunch {
-  uint64_t units;  // of all tensors
+  uint32_t tiles;  // of all tensors
   int32_t n;
+  int32_t all_in_place;
   int32_t reserved;
   GradDesc d[CAP];
 };
-
-struct GradList {  // host side: the descriptors of one launch
-  const GradDesc* d;
-  int n;
-  uint64_t units;
+// What folding the tensors' own norms needs of them.
+template <int CAP>
+struct FoldLaunch {
+  uint32_t tiles;
+  int32_t n;
+  struct {
+    uint32_t t_begin, id;
+  } d[CAP];
 };
 
-// Blocks that the norm of `units` units is split over (0: no device).
-int norm_blocks(uint64_t units);
+struct GradPart {  // host side: one launch
+  int g_dtype = TK_F32;
+  int n = 0;
+  uint32_t tiles = 0;
+  uint64_t units = 0;
+  int cap = 0;                          // 64, 320 or kMaxGrads
+  std::unique_ptr<uint64_t[]> launch;   // GradLaunch<cap>
+  std::unique_ptr<uint64_t[]> fold;     // FoldLaunch<cap>
+  int build(int g_dtype, const GradDesc* d, int n, uint32_t tiles);
+};
 
-// Sum of powers (or largest magnitude) of every block's share into
-// partials[0..blocks); with `slots`, also block b's share of tensor i into
-// slots[b + i].
-int launch_norm(const GradList& l, int norm, int blocks, double* partials, double* slots,
-                cudaStream_t s);
-// out = out + alpha g, or alpha g; norm < 0: without the norm.
-int launch_sum(const GradList& l, int norm, float alpha, bool overwrite, int blocks,
-               double* partials, cudaStream_t s);
-// Norm and clip scale of the partials (norm_out, scale_out may be null).
-int launch_fold(int norm, const double* partials, int n, float max_norm, float* norm_out,
-                float* scale_out, cudaStream_t s);
-// Norm of each tensor of one launch from its slots.
-int launch_fold_each(const GradList& l, int norm, int blocks, const double* slots, float* each,
-                     cudaStream_t s);
-// out = scale g with the scale of the partials.
-int launch_clip(const GradList& l, int norm, const double* partials, int n, float max_norm,
-                float* norm_out, float* scale_out, cudaStream_t s);
+inline uint64_t tiles_of(int g_dtype, uint64_t phase, uint64_t n) {
+  const uint64_t per = (uint64_t)kUnit * (g_dtype == TK_F32 ? kTileUnits<TK_F32> : kTileUnits<TK_BF16>);
+  return n ? (phase + n + per - 1) / per : 0;
+}
+
+// Sum of powers (or largest magnitude) of each tile into partials[0..p.tiles).
+int launch_norm(const GradPart& p, int norm, double* partials, cudaStream_t s);
+// out = out + alpha g, or alpha g, and the same of each tile of the new out;
+// norm TK_NORM_NONE: without it.
+int launch_sum(const GradPart& p, int norm, float alpha, bool overwrite, double* partials,
+               cudaStream_t s);
+
+// The norm and its clip scale, each where it is not null.
+struct NormOut {
+  float max_norm = 0.0f;
+  float* norm = nullptr;
+  float* scale = nullptr;
+  float* scale_too = nullptr;
+};
+// Both from n partials.  Enqueued right behind the launches that write them.
+int launch_fold(int norm, const double* partials, int64_t n, const NormOut& out, cudaStream_t s);
+// Norm of each tensor of one part from its partials, into each[id]; with out,
+// the norm of n partials from `all` too.
+int launch_fold_each(const GradPart& p, int norm, const double* partials, float* each,
+                     const double* all, int64_t n, const NormOut* out, cudaStream_t s);
+// out = *scale g.  Enqueued right behind the launch that writes *scale.
+int launch_clip(const GradPart& p, const float* scale, cudaStream_t s);
+
+// A whole call in one launch, for a table of one part and few tiles (small).
+bool small(const GradPart& p);
+enum { SMALL_NORM = 0, SMALL_CLIP = 1, SMALL_SUM = 2, SMALL_FIRST = 3 };
+int launch_small(const GradPart& p, int op, int norm, float alpha, const NormOut& out,
+                 cudaStream_t s);
 
 }  // namespace gr
 }  // namespace tk

@@ -14,19 +14,14 @@ struct tk_grad_table {
   size_t n = 0;
   bool can_clip = false;  // no buffer that clipping writes shares memory with another
   bool can_sum = false;   // every out is f32 and not its own g
-  std::vector<tk::gr::GradDesc> d;
-  struct Part {
-    size_t first;
-    int n;
-    uint64_t units;
-  };
-  std::vector<Part> parts;  // one launch each
+  std::vector<tk::gr::GradPart> parts;  // one launch each
 };
 
 namespace tk {
 namespace {
 
-constexpr uint64_t kMaxElems = 1ull << 40;  // units * blocks stays far inside 64 bits
+constexpr uint64_t kMaxElems = 1ull << 40;  // of one tensor; a descriptor holds 44 bits
+constexpr uint64_t kMaxTiles = 1ull << 28;  // of one table; a tile's number has 32 bits, a grid's 31
 
 size_t size_of(int dt) { return dt == TK_F32 ? 4 : 2; }
 bool known(int dt) { return dt == TK_F32 || dt == TK_BF16 || dt == TK_F16; }
@@ -40,6 +35,18 @@ int check_address(size_t i, const char* what, const void* p, int dt) {
     return set_error(TK_ERR_INVALID, "gradient %zu: %s at %p is not aligned to its element size", i,
                      what, p);
   return TK_OK;
+}
+
+struct Target {
+  uintptr_t at;
+  int dtype;
+  bool in_place;
+};
+
+Target target_of(const tk_grad& g) {
+  if (g.out == nullptr || (g.out == g.g && g.out_dtype == g.g_dtype))
+    return {(uintptr_t)g.g, g.g_dtype, true};
+  return {(uintptr_t)g.out, g.out_dtype, false};
 }
 
 int check_device(size_t i, const char* what, const void* p, int dev) {
@@ -57,7 +64,6 @@ int create(const tk_grad* grads, size_t n, tk_grad_table** out) {
   auto t = std::make_unique<tk_grad_table>();
   t->n = n;
   t->can_sum = true;
-  t->d.reserve(n);
   // A gradient in place counts as read only in `ranges`, as written in
   // `clipped`: a norm may be taken of one tensor given twice, but clipping it
   // would scale it twice.
@@ -65,44 +71,25 @@ int create(const tk_grad* grads, size_t n, tk_grad_table** out) {
   uint64_t total = 0;
   for (size_t i = 0; i < n; ++i) {
     const tk_grad& g = grads[i];
-    gr::GradDesc d = {};
-    if (g.n > 0) {
-      if (g.n > kMaxElems)
-        return set_error(TK_ERR_INVALID, "gradient %zu: %llu elements are too many", i,
-                         (unsigned long long)g.n);
-      TK_TRY(check_address(i, "g", g.g, g.g_dtype));
-      if (g.out != nullptr) TK_TRY(check_address(i, "out", g.out, g.out_dtype));
-      const bool same = g.out == nullptr || (g.out == g.g && g.out_dtype == g.g_dtype);
-      const uintptr_t ga = (uintptr_t)g.g, oa = same ? ga : (uintptr_t)g.out;
-      const int odt = same ? g.g_dtype : g.out_dtype;
-      const size_t ge = size_of(g.g_dtype), oe = size_of(odt);
-      ranges.push_back({ga, ga + g.n * ge, false});
-      clipped.push_back({ga, ga + g.n * ge, same});
-      if (!same) {
-        ranges.push_back({oa, oa + g.n * oe, true});
-        clipped.push_back(ranges.back());
-      }
-      if (same || odt != TK_F32) t->can_sum = false;
-      const uint64_t phase = ga / ge % gr::kUnit;
-      d.g = reinterpret_cast<const char*>(ga - phase * ge);
-      d.out = reinterpret_cast<char*>(oa - phase * oe);
-      d.n = g.n;
-      d.phase = phase;
-      d.g_dtype = (uint64_t)g.g_dtype;
-      d.out_dtype = (uint64_t)odt;
-      d.out_vec = oa / oe % gr::kUnit == phase;
-      d.in_place = same;
-      const uint64_t units = (phase + g.n + gr::kUnit - 1) / gr::kUnit;
-      total += units;
-      if (total > kMaxElems)
-        return set_error(TK_ERR_INVALID, "the gradients have too many elements for one table");
+    if (g.n == 0) continue;
+    if (g.n > kMaxElems)
+      return set_error(TK_ERR_INVALID, "gradient %zu: %llu elements are too many", i,
+                       (unsigned long long)g.n);
+    TK_TRY(check_address(i, "g", g.g, g.g_dtype));
+    if (g.out != nullptr) TK_TRY(check_address(i, "out", g.out, g.out_dtype));
+    const Target o = target_of(g);
+    const uintptr_t ga = (uintptr_t)g.g;
+    ranges.push_back({ga, ga + g.n * size_of(g.g_dtype), false});
+    clipped.push_back(ranges.back());
+    clipped.back().writable = o.in_place;
+    if (!o.in_place) {
+      ranges.push_back({o.at, o.at + g.n * size_of(o.dtype), true});
+      clipped.push_back(ranges.back());
     }
-    if (t->parts.empty() || t->parts.back().n == gr::kMaxGrads) t->parts.push_back({i, 0, 0});
-    tk_grad_table::Part& p = t->parts.back();
-    d.u_begin = p.units;
-    p.units += d.n ? (d.phase + d.n + gr::kUnit - 1) / gr::kUnit : 0;
-    ++p.n;
-    t->d.push_back(d);
+    if (o.in_place || o.dtype != TK_F32) t->can_sum = false;
+    total += gr::tiles_of(g.g_dtype, gr::kUnit, g.n);
+    if (total > kMaxTiles)
+      return set_error(TK_ERR_INVALID, "the gradients have too many elements for one table");
   }
   TK_TRY(check_overlaps(ranges.data(), ranges.size()));
   t->can_clip = check_overlaps(clipped.data(), clipped.size()) == TK_OK;
@@ -112,6 +99,42 @@ int create(const tk_grad* grads, size_t n, tk_grad_table** out) {
     if (grads[i].n == 0) continue;
     TK_TRY(check_device(i, "g", grads[i].g, t->dev));
     if (grads[i].out != nullptr) TK_TRY(check_device(i, "out", grads[i].out, t->dev));
+  }
+  // One type after the other: a kernel is compiled for each, and a part has
+  // one.  Empty gradients go with the first; their own norms are 0.
+  for (const int dt : {TK_F32, TK_BF16, TK_F16}) {
+    std::vector<gr::GradDesc> d;
+    uint32_t tiles = 0;
+    auto close = [&] {
+      if (d.empty()) return;
+      t->parts.emplace_back();
+      t->parts.back().build(dt, d.data(), (int)d.size(), tiles);
+      d.clear();
+      tiles = 0;
+    };
+    for (size_t i = 0; i < n; ++i) {
+      const tk_grad& g = grads[i];
+      if (g.n == 0 ? dt != TK_F32 : g.g_dtype != dt) continue;
+      gr::GradDesc x = {};
+      x.t_begin = tiles;
+      x.id = (uint32_t)i;
+      if (g.n > 0) {
+        const Target o = target_of(g);
+        const uintptr_t ga = (uintptr_t)g.g;
+        const uint64_t phase = ga / size_of(dt) % gr::kUnit;
+        x.g = reinterpret_cast<const char*>(ga - phase * size_of(dt));
+        x.out = reinterpret_cast<char*>(o.at - phase * size_of(o.dtype));
+        x.n = g.n;
+        x.phase = phase;
+        x.out_dtype = (uint64_t)o.dtype;
+        x.out_vec = o.at / size_of(o.dtype) % gr::kUnit == phase;
+        x.in_place = o.in_place;
+        tiles += (uint32_t)gr::tiles_of(dt, phase, g.n);
+      }
+      d.push_back(x);
+      if (d.size() == gr::kMaxGrads) close();
+    }
+    close();
   }
   *out = t.release();
   return TK_OK;
@@ -130,94 +153,81 @@ int check_call(const tk_grad_table* t, int norm, bool none_ok) {
   return TK_OK;
 }
 
-gr::GradList list_of(const tk_grad_table& t, const tk_grad_table::Part& p) {
-  return {t.d.data() + p.first, p.n, p.units};
+size_t tiles_of(const tk_grad_table& t) {
+  size_t n = 0;
+  for (const auto& p : t.parts) n += p.tiles;
+  return n;
 }
 
-// Blocks of each part's norm, and of all.
-int norm_plan(const tk_grad_table& t, std::vector<int>* blocks, int* total) {
-  *total = 0;
+// Every part's partials, one after the other.
+int norm_parts(const tk_grad_table& t, int norm, double* partials, cudaStream_t s) {
   for (const auto& p : t.parts) {
-    const int b = p.units ? gr::norm_blocks(p.units) : 0;
-    if (p.units && b <= 0) return set_error(TK_ERR_CUDA, "could not size the norm grid");
-    blocks->push_back(b);
-    *total += b;
+    if (p.tiles) TK_TRY(gr::launch_norm(p, norm, partials, s));
+    partials += p.tiles;
   }
   return TK_OK;
 }
 
-int grad_norm(const tk_grad_table& t, int norm, float max_norm, float* norm_dev, float* each_dev,
-              float* scale_dev, cudaStream_t s) {
-  NvtxRange r("tikun/grad_norm");
-  std::vector<int> blocks;
-  int total = 0;
-  TK_TRY(norm_plan(t, &blocks, &total));
-  Scratch sc;
-  // partials of every part, and behind them each part's blocks + n slots
-  TK_TRY(sc.alloc(sizeof(double) * (total + (each_dev ? total + t.n : 0) + 1), s));
-  double* partials = static_cast<double*>(sc.get());
-  double* slots = partials + total;
-  int at = 0;
-  for (size_t i = 0; i < t.parts.size(); ++i) {
-    const auto& p = t.parts[i];
-    const gr::GradList l = list_of(t, p);
-    if (p.units) TK_TRY(gr::launch_norm(l, norm, blocks[i], partials + at, each_dev ? slots : nullptr, s));
-    if (each_dev) {
-      TK_TRY(gr::launch_fold_each(l, norm, blocks[i], slots, each_dev + p.first, s));
-      slots += blocks[i] + p.n;
-    }
-    at += blocks[i];
-  }
-  if (norm_dev == nullptr && scale_dev == nullptr) return TK_OK;
-  return gr::launch_fold(norm, partials, total, max_norm, norm_dev, scale_dev, s);
-}
+bool small(const tk_grad_table& t) { return t.parts.size() == 1 && gr::small(t.parts[0]); }
 
-int clip_grad_norm(const tk_grad_table& t, int norm, float max_norm, float* norm_dev,
-                   float* scale_dev, cudaStream_t s) {
-  NvtxRange r("tikun/clip_grad_norm");
-  std::vector<int> blocks;
-  int total = 0;
-  TK_TRY(norm_plan(t, &blocks, &total));
-  if (total == 0) return grad_norm(t, norm, max_norm, norm_dev, nullptr, scale_dev, s);
+int grad_norm(const tk_grad_table& t, int norm, const gr::NormOut& out, float* each_dev,
+              cudaStream_t s) {
+  NvtxRange r("tikun/grad_norm");
+  if (each_dev == nullptr && small(t))
+    return gr::launch_small(t.parts[0], gr::SMALL_NORM, norm, 0.0f, out, s);
+  const size_t total = tiles_of(t);
   Scratch sc;
   TK_TRY(sc.alloc(sizeof(double) * total, s));
   double* partials = static_cast<double*>(sc.get());
-  int at = 0;
-  for (size_t i = 0; i < t.parts.size(); ++i) {
-    if (blocks[i]) TK_TRY(gr::launch_norm(list_of(t, t.parts[i]), norm, blocks[i], partials + at, nullptr, s));
-    at += blocks[i];
+  TK_TRY(norm_parts(t, norm, partials, s));
+  if (each_dev == nullptr || t.parts.empty())
+    return gr::launch_fold(norm, partials, (int64_t)total, out, s);
+  const double* at = partials;
+  for (const auto& p : t.parts) {  // with the last one, the norm of all
+    TK_TRY(gr::launch_fold_each(p, norm, at, each_dev, partials, (int64_t)total,
+                                &p == &t.parts.back() ? &out : nullptr, s));
+    at += p.tiles;
   }
-  bool first = true;
-  for (const auto& p : t.parts) {
-    if (!p.units) continue;
-    TK_TRY(gr::launch_clip(list_of(t, p), norm, partials, total, max_norm,
-                           first ? norm_dev : nullptr, first ? scale_dev : nullptr, s));
-    first = false;
-  }
+  return TK_OK;
+}
+
+int clip_grad_norm(const tk_grad_table& t, int norm, gr::NormOut out, cudaStream_t s) {
+  NvtxRange r("tikun/clip_grad_norm");
+  if (small(t)) return gr::launch_small(t.parts[0], gr::SMALL_CLIP, norm, 0.0f, out, s);
+  const size_t total = tiles_of(t);
+  Scratch sc;
+  TK_TRY(sc.alloc(sizeof(double) * (total + 1), s));
+  double* partials = static_cast<double*>(sc.get());
+  out.scale_too = reinterpret_cast<float*>(partials + total);
+  TK_TRY(norm_parts(t, norm, partials, s));
+  TK_TRY(gr::launch_fold(norm, partials, (int64_t)total, out, s));
+  for (size_t i = t.parts.size(); i-- > 0;)  // the norm's last part first
+    if (t.parts[i].tiles) TK_TRY(gr::launch_clip(t.parts[i], out.scale_too, s));
   return TK_OK;
 }
 
 int accumulate(const tk_grad_table& t, float alpha, bool overwrite, int norm, float* norm_dev,
                cudaStream_t s) {
   NvtxRange r("tikun/accumulate_grads");
-  std::vector<int> blocks;
-  int total = 0;
-  TK_TRY(norm_plan(t, &blocks, &total));
+  gr::NormOut out;
+  out.norm = norm_dev;
+  const bool with = norm != TK_NORM_NONE;
+  if (with && small(t))
+    return gr::launch_small(t.parts[0], overwrite ? gr::SMALL_FIRST : gr::SMALL_SUM, norm, alpha,
+                            out, s);
+  const size_t total = tiles_of(t);
   Scratch sc;
   double* partials = nullptr;
-  if (norm != TK_NORM_NONE) {
-    TK_TRY(sc.alloc(sizeof(double) * (total + 1), s));
+  if (with) {
+    TK_TRY(sc.alloc(sizeof(double) * total, s));
     partials = static_cast<double*>(sc.get());
   }
-  int at = 0;
-  for (size_t i = 0; i < t.parts.size(); ++i) {
-    if (blocks[i])
-      TK_TRY(gr::launch_sum(list_of(t, t.parts[i]), norm, alpha, overwrite, blocks[i],
-                            partials ? partials + at : nullptr, s));
-    at += blocks[i];
+  double* at = partials;
+  for (const auto& p : t.parts) {
+    if (p.tiles) TK_TRY(gr::launch_sum(p, norm, alpha, overwrite, at, s));
+    if (with) at += p.tiles;
   }
-  if (norm == TK_NORM_NONE) return TK_OK;
-  return gr::launch_fold(norm, partials, total, 0.0f, norm_dev, nullptr, s);
+  return with ? gr::launch_fold(norm, partials, (int64_t)total, out, s) : TK_OK;
 }
 
 // No C++ exception leaves a C entry point.
@@ -252,7 +262,7 @@ int tk_grad_norm(const tk_grad_table* table, int32_t norm, float max_norm, float
                  float* each_dev, float* scale_dev, void* stream) {
   return guarded([&] {
     TK_TRY(check_call(table, norm, false));
-    return grad_norm(*table, norm, max_norm, norm_dev, each_dev, scale_dev,
+    return grad_norm(*table, norm, {max_norm, norm_dev, scale_dev, nullptr}, each_dev,
                      static_cast<cudaStream_t>(stream));
   });
 }
@@ -266,7 +276,7 @@ int tk_clip_grad_norm(const tk_grad_table* table, int32_t norm, float max_norm, 
     if (!table->can_clip)
       return set_error(TK_ERR_INVALID, "a gradient that is clipped in place shares memory with "
                        "another buffer of the table");
-    return clip_grad_norm(*table, norm, max_norm, norm_dev, scale_dev,
+    return clip_grad_norm(*table, norm, {max_norm, norm_dev, scale_dev, nullptr},
                           static_cast<cudaStream_t>(stream));
   });
 }

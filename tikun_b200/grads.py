@@ -23,6 +23,7 @@ CUDA graph.  No call is seen by autograd.
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import math
 
@@ -37,7 +38,7 @@ _DTYPES = {torch.float32: _native.TK_F32, torch.bfloat16: _native.TK_BF16,
 
 
 def _norm_code(norm_type) -> int:
-    code = _NORMS.get(float(norm_type))
+    code = _NORMS.get(norm_type)
     if code is None:
         raise ValueError(f"norm_type is 2, 1 or inf, got {norm_type!r}")
     return code
@@ -55,7 +56,8 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
-def _check(t, what: str) -> None:
+def _refuse(t, what: str) -> None:
+    """Raises for what is not a dense CUDA tensor of one of the types."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{what}: expected a torch tensor, got {type(t).__name__}")
     if t.layout != torch.strided or not t.is_cuda:
@@ -65,6 +67,52 @@ def _check(t, what: str) -> None:
     if t.numel() and not _dense(t):
         raise ValueError(f"{what}: its elements do not fill one stretch of memory (shape "
                          f"{tuple(t.shape)}, strides {t.stride()})")
+
+
+def _columns(ts: list, what: str) -> tuple[list, list, list, set]:
+    """Addresses, element counts and type codes of checked tensors, and their
+    device indices.  One attribute of all tensors at a time, which takes a third
+    of the time of one tensor at a time."""
+    try:
+        plain = all([t.is_contiguous() for t in ts]) and all([t.is_cuda for t in ts]) and \
+            all([t.layout is torch.strided for t in ts])
+        codes = [_DTYPES[t.dtype] for t in ts]
+    except (AttributeError, KeyError, RuntimeError):
+        plain, codes = False, None
+    if not plain:
+        for i, t in enumerate(ts):
+            _refuse(t, f"{what} {i}")
+        codes = [_DTYPES[t.dtype] for t in ts]
+    return ([t.data_ptr() for t in ts], [t.numel() for t in ts], codes,
+            {t.get_device() for t in ts})
+
+
+# what current_stream().cuda_stream gives, at a fortieth of its 3 us
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _stream(index: int) -> int:
+    if _raw_stream is not None:
+        return _raw_stream(index)
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+def _on_device(t: "GradTable", call):
+    """call(stream) with the table's device current."""
+    index = t.device.index
+    if torch.cuda.current_device() == index:
+        return call(_stream(index))
+    with torch.cuda.device(index):
+        return call(_stream(index))
+
+
+def _leaves(tree) -> list:
+    """flatten_leaves, without its walk for a plain list of tensors."""
+    if not isinstance(tree, (list, tuple, dict, torch.Tensor)) and hasattr(tree, "__iter__"):
+        tree = list(tree)  # model.parameters()
+    if isinstance(tree, (list, tuple)) and all([isinstance(t, torch.Tensor) for t in tree]):
+        return list(tree)
+    return flatten_leaves(tree)
 
 
 class GradTable:
@@ -80,50 +128,52 @@ class GradTable:
     def __init__(self, grads, out=None):
         self._handle = None
         self._params = []
-        self.grads = []
-        for leaf in flatten_leaves(grads):
-            if isinstance(leaf, torch.nn.Parameter):
-                if leaf.grad is None:
-                    continue
-                self._params.append((leaf, leaf.grad))
-                leaf = leaf.grad
-            elif leaf is None:
-                continue
-            _check(leaf, f"gradient {len(self.grads)}")
-            self.grads.append(leaf)
-        self.out = None if out is None else flatten_leaves(out)
+        self.grads = _leaves(grads)
+        # a plain tensor is no Parameter (whose isinstance costs ten times as much)
+        if not all([type(t) is torch.Tensor for t in self.grads]):
+            leaves, self.grads = self.grads, []
+            for leaf in leaves:
+                if isinstance(leaf, torch.nn.Parameter):
+                    g = leaf.grad
+                    if g is not None:
+                        self._params.append((leaf, g))
+                        self.grads.append(g)
+                elif leaf is not None:
+                    self.grads.append(leaf)
         n = len(self.grads)
-        if self.out is not None:
+        at, sizes, codes, devices = _columns(self.grads, "gradient")
+        out_at = [0] * n
+        self.out = None
+        if out is not None:
+            self.out = _leaves(out)
             if len(self.out) != n:
                 raise ValueError(f"{len(self.out)} out tensors for {n} gradients")
+            out_at, out_sizes, out_codes, out_devices = _columns(self.out, "out")
+            devices |= out_devices
+            codes = [g | o << 32 for g, o in zip(codes, out_codes)]  # the C struct's two int32
             for i, (g, o) in enumerate(zip(self.grads, self.out)):
-                _check(o, f"out {i}")
-                if o.numel() != g.numel() or not (
-                        g.is_contiguous() and o.is_contiguous() or o.stride() == g.stride()):
+                if out_sizes[i] != sizes[i] or not (g.is_contiguous() and o.is_contiguous() or
+                                                    o.stride() == g.stride()):
                     raise ValueError(f"out {i} has shape {tuple(o.shape)} and strides "
                                      f"{o.stride()}, its gradient {tuple(g.shape)} and "
                                      f"{g.stride()}")
-        devices = {t.device for t in self.grads + (self.out or [])}
         if len(devices) > 1:
-            raise ValueError("the tensors of one call are on one device, got "
-                             f"{sorted(map(str, devices))}")
-        self.device = devices.pop() if devices else torch.device("cuda", torch.cuda.current_device())
-        arr = (_native.TkGrad * max(n, 1))()
-        for i, g in enumerate(self.grads):
-            o = self.out[i] if self.out is not None else None
-            arr[i] = _native.TkGrad(g.data_ptr(), 0 if o is None else o.data_ptr(), g.numel(),
-                                    _DTYPES[g.dtype], 0 if o is None else _DTYPES[o.dtype])
+            raise ValueError(f"the tensors of one call are on one device, got {sorted(devices)}")
+        self.device = torch.device("cuda", devices.pop() if devices else torch.cuda.current_device())
+        words = array.array("Q", [w for row in zip(at, out_at, sizes, codes) for w in row])
+        entries = ctypes.cast(words.buffer_info()[0], ctypes.POINTER(_native.TkGrad))
         handle = ctypes.c_void_p()
-        with torch.cuda.device(self.device):
-            _native.check(_native.lib().tk_grad_table_create(arr, n, ctypes.byref(handle)))
+        _on_device(self, lambda _: _native.check(
+            _native.lib().tk_grad_table_create(entries, n, ctypes.byref(handle))))
         self._handle = handle
+        self._destroy = _native.lib().tk_grad_table_destroy
 
     def __len__(self) -> int:
         return len(self.grads)
 
     def __del__(self):
-        if getattr(self, "_handle", None) is not None:
-            _native.lib().tk_grad_table_destroy(self._handle)
+        if self._handle is not None:
+            self._destroy(self._handle)
             self._handle = None
 
     def _standing(self) -> "GradTable":
@@ -152,19 +202,18 @@ def grad_norm(grads, norm_type: float = 2.0, per_tensor: bool = False,
               error_if_nonfinite: bool = False):
     """The norm of all gradients' elements as one vector, a 0-dim f32 tensor:
     sqrt(sum x^2) (2), sum |x| (1) or max |x| (``inf``); 0 without elements,
-    NaN with a NaN among them.  Sums are formed in f64 in a fixed order and
-    rounded once.
+    NaN with a NaN among them.  Sums are formed in f64 (of bf16 and f16 values
+    first by eights in f32) in a fixed order and rounded once.
 
     ``per_tensor=True``: (norm, norms), ``norms`` the f32 norms of the
     gradients, one each."""
     code = _norm_code(norm_type)
     t = _table(grads)
-    with torch.cuda.device(t.device):
-        norm = torch.empty((), dtype=torch.float32, device=t.device)
-        each = torch.empty(len(t), dtype=torch.float32, device=t.device) if per_tensor else None
-        _native.check(_native.lib().tk_grad_norm(
-            t._handle, code, 0.0, norm.data_ptr(), each.data_ptr() if len(t) and per_tensor else None,
-            None, torch.cuda.current_stream().cuda_stream))
+    norm = torch.empty((), dtype=torch.float32, device=t.device)
+    each = torch.empty(len(t), dtype=torch.float32, device=t.device) if per_tensor else None
+    each_ptr = each.data_ptr() if per_tensor and len(t) else None
+    _on_device(t, lambda stream: _native.check(_native.lib().tk_grad_norm(
+        t._handle, code, 0.0, norm.data_ptr(), each_ptr, None, stream)))
     if error_if_nonfinite:
         _finite(norm, norm_type)
     return (norm, each) if per_tensor else norm
@@ -187,15 +236,11 @@ def clip_grad_norm_(grads, max_norm: float, norm_type: float = 2.0, out=None,
     if not max_norm > 0:
         raise ValueError(f"max_norm is positive, got {max_norm!r}")
     t = _table(grads, out)
-    with torch.cuda.device(t.device):
-        norm = torch.empty((), dtype=torch.float32, device=t.device)
-        stream = torch.cuda.current_stream().cuda_stream
-        if error_if_nonfinite:
-            _native.check(_native.lib().tk_grad_norm(t._handle, code, 0.0, norm.data_ptr(), None,
-                                                     None, stream))
-            _finite(norm, norm_type)
-        _native.check(_native.lib().tk_clip_grad_norm(t._handle, code, max_norm, norm.data_ptr(),
-                                                      None, stream))
+    if error_if_nonfinite:
+        grad_norm(t, norm_type, error_if_nonfinite=True)
+    norm = torch.empty((), dtype=torch.float32, device=t.device)
+    _on_device(t, lambda stream: _native.check(_native.lib().tk_clip_grad_norm(
+        t._handle, code, max_norm, norm.data_ptr(), None, stream)))
     return norm
 
 
@@ -213,11 +258,10 @@ def accumulate_grads_(grads, acc=None, alpha: float = 1.0, overwrite: bool = Fal
     if not isinstance(grads, GradTable) and acc is None:
         raise ValueError("accumulate_grads_ needs acc")
     t = _table(grads, acc)
-    with torch.cuda.device(t.device):
-        norm = torch.empty((), dtype=torch.float32, device=t.device) if norm_type is not None else None
-        _native.check(_native.lib().tk_accumulate_grads(
-            t._handle, alpha, 1 if overwrite else 0, code,
-            norm.data_ptr() if norm is not None else None, torch.cuda.current_stream().cuda_stream))
+    norm = torch.empty((), dtype=torch.float32, device=t.device) if norm_type is not None else None
+    norm_ptr = norm.data_ptr() if norm is not None else None
+    _on_device(t, lambda stream: _native.check(_native.lib().tk_accumulate_grads(
+        t._handle, alpha, 1 if overwrite else 0, code, norm_ptr, stream)))
     return norm
 
 
