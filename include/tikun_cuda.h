@@ -333,6 +333,13 @@ typedef struct {
 TK_API int tk_muon_step(const tk_muon_leaf* leaves, size_t n_leaves,
                         const tk_muon_hparams* hp, void* stream);
 
+/* tk_muon_step over device leaves with every gradient multiplied by the clip
+ * scale at scale_dev (device memory, as tk_grad_norm forms it), in f32 and in
+ * the prologue pass that reads the gradients anyway: a clip by one norm over
+ * the leaves of this call and of others. */
+TK_API int tk_muon_step_clipped(const tk_muon_leaf* leaves, size_t n_leaves,
+                                const tk_muon_hparams* hp, const float* scale_dev, void* stream);
+
 /* Waits for the device, then reads and clears its status word (0: no kernel
  * reported a problem). */
 TK_API int tk_device_status(int* status_out);

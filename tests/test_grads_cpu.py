@@ -82,3 +82,17 @@ def test_dense_views():
         assert grads._dense(v)
     for v in (t[:, ::2], t[:, 1:], t[..., 0], torch.zeros(3, 1).expand(3, 4)):
         assert not grads._dense(v)
+
+
+def test_clip_scale_is_refused_before_a_step():
+    p = torch.nn.Parameter(torch.zeros(3))
+    p.grad = torch.ones(3)
+    for opt in (tikun_b200.AdamW([p]), tikun_b200.MuonND([p]), tikun_b200.Muon([p])):
+        for bad in (0.5, torch.tensor(0.5)):
+            with pytest.raises(ValueError, match="one float32 value on a CUDA device"):
+                opt.step(clip_scale=bad)
+        assert opt.step_count == 0
+    with pytest.raises(ValueError, match="max_norm is positive"):
+        tikun_b200.clip_scale([p], 0.0)
+    with pytest.raises(ValueError, match="expected a dense CUDA tensor"):
+        tikun_b200.MuonND([p], max_norm=1.0).step()

@@ -354,6 +354,118 @@ def test_micro_batches_norm_clip_and_step_together():
         assert ((t.double() - want).abs() <= 8 * U * x.abs().max() + 2.0 ** -149).all()
 
 
+def muon_params(seed=3):
+    gen = torch.Generator().manual_seed(seed)
+    shapes = [(256, 384), (384, 256), (96, 40), (3, 64, 32), (768,), (5,)]
+    return [torch.randn(s, generator=gen).cuda() * 0.02 for s in shapes]
+
+
+@pytest.mark.parametrize("over", [True, False], ids=["over", "under"])
+@pytest.mark.parametrize("dtype", DTYPES[:2], ids=IDS[:2])
+def test_muon_nd_clips_by_the_common_norm(dtype, over):
+    """Three clipped steps give the bits of steps on gradients multiplied by
+    the scale in f32, which is what the norm of all leaves calls for."""
+    a = [torch.nn.Parameter(t) for t in muon_params()]
+    b = [torch.nn.Parameter(t.clone()) for t in muon_params()]
+    opt_a = tikun_b200.MuonND(a, max_norm=0.01 if over else 100.0)
+    opt_b = tikun_b200.MuonND(b)
+    for step in range(3):
+        gs = [t.to(dtype) * 0.1 for t in muon_params(seed=10 + step)]
+        for p, g in zip(a, gs):
+            p.grad_dtype = None  # it may have another type than its parameter
+            p.grad = g
+        opt_a.step()
+        want = norm64(gs, 2.0)
+        assert_norm(opt_a.grad_norm, want, dtype, 2.0)
+        scale = opt_a.clip_scale.cpu()
+        assert (scale.item() < 1.0) == over
+        for p, g in zip(b, gs):
+            p.grad = (g.cpu().float() * scale).cuda()
+        opt_b.step()
+        for x, y, g in zip(a, b, gs):
+            assert same_bits(x, y)
+            assert same_bits(x.grad, g)  # the gradients stay as they are
+
+
+def test_muon_clips_its_two_groups_together():
+    def build(**kw):
+        ps = [torch.nn.Parameter(t) for t in muon_params()]
+        return ps, tikun_b200.Muon(ps[:3], ps[4:], **kw)
+
+    a, opt_a = build(max_norm=0.05)
+    b, opt_b = build()
+    c, opt_c = build()
+    used = [0, 1, 2, 4, 5]
+    for step in range(2):
+        gs = [t * 0.1 for t in muon_params(seed=20 + step)]
+        for i in used:
+            a[i].grad, c[i].grad = gs[i].clone(), gs[i].clone()
+        opt_a.step()
+        assert_norm(opt_a.grad_norm, norm64([gs[i] for i in used], 2.0), torch.float32, 2.0)
+        norm, scale = tikun_b200.clip_scale([gs[i] for i in used], 0.05)
+        assert same_bits(norm, opt_a.grad_norm) and same_bits(scale, opt_a.clip_scale)
+        assert scale.item() == (np.float32(0.05) / (np.float32(norm.item()) + np.float32(1e-6)))
+        opt_c.step(clip_scale=scale)
+        for i in used:
+            b[i].grad = gs[i] * scale
+        opt_b.step()
+        for i in used:
+            assert same_bits(a[i], b[i]) and same_bits(c[i], b[i])
+
+
+@pytest.mark.parametrize("form", ["adamw", "lion", "sgd", "arena", "torch-adamw"])
+def test_optimizers_take_a_common_scale(form):
+    from tikun_b200.optimizer import AdamW as TorchAdamW
+
+    def build(ts):
+        ps = [torch.nn.Parameter(t.clone()) for t in ts]
+        if form == "torch-adamw":
+            return ps, TorchAdamW(ps)
+        if form == "arena":
+            return ps, tikun_b200.AdamW(ps, arena=True)
+        return ps, tikun_b200.Optimizer(ps, algorithm=form)
+
+    ts = muon_params()
+    (a, opt_a), (b, opt_b) = build(ts), build(ts)
+    other = torch.randn(1000, device="cuda")
+    for step in range(2):
+        gs = [t * 0.1 for t in muon_params(seed=30 + step)]
+        norm, scale = tikun_b200.clip_scale([gs, other], 0.5)
+        assert_norm(norm, norm64(gs + [other], 2.0), torch.float32, 2.0)
+        assert scale.item() < 1.0
+        for p, q, g in zip(a, b, gs):
+            if form == "arena":
+                p.grad.copy_(g)
+                q.grad.copy_(g * scale)
+            else:
+                p.grad, q.grad = g, g * scale
+        opt_a.step(clip_scale=scale)
+        opt_b.step()
+        for x, y in zip(a, b):
+            assert same_bits(x, y)
+    with pytest.raises(ValueError, match="one float32 value"):
+        opt_a.step(clip_scale=scale.double())
+
+
+def test_clip_scale_refusals():
+    p = torch.nn.Parameter(torch.zeros(8, device="cuda"))
+    p.grad = torch.ones(8, device="cuda")
+    norm, scale = tikun_b200.clip_scale([p], 1.0)
+    for opt in (tikun_b200.AdamW([p], max_norm=1.0), tikun_b200.MuonND([p], max_norm=1.0)):
+        with pytest.raises(ValueError, match="forms its own clip scale"):
+            opt.step(clip_scale=scale)
+    with pytest.raises(ValueError, match="before a common norm is known"):
+        tikun_b200.AdamW([p], in_backward=True).step(clip_scale=scale)
+    w = np.zeros((4, 4), np.float32)
+    leaf = (_native.TkMuonLeaf * 1)(_native.TkMuonLeaf(w.ctypes.data, w.ctypes.data + 16,
+                                                      w.ctypes.data + 32, 1, 2, 2, 0, 0))
+    hp = _native.TkMuonHParams(0.02, 0.95, 1, 5, _native.TK_NS_F16)
+    L = _native.lib()
+    for ptr, text in ((None, "scale_dev is NULL"), (scale.data_ptr(), "takes device buffers")):
+        with pytest.raises(ValueError, match=text):
+            _native.check(L.tk_muon_step_clipped(leaf, 1, ctypes.byref(hp), ptr, None))
+
+
 def test_captured_calls_and_graphs_side_by_side():
     """Two captured graphs on two streams, replayed at once on new contents,
     beside eager calls on a third."""

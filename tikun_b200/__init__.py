@@ -6,7 +6,8 @@ Front-ends with the reference's names and arguments (python/tikun/__init__.py):
 entry points of the reference's ``_tikun`` module are in ``tikun_b200._native``.
 
 Beside them, for the gradients between backward and step (``tikun_b200.grads``):
-``grad_norm``, ``clip_grad_norm_``, ``accumulate_grads_`` and ``GradTable``.
+``grad_norm``, ``clip_scale``, ``clip_grad_norm_``, ``accumulate_grads_`` and
+``GradTable``.
 """
 from .universal import UniversalOptimizer as Optimizer
 from .universal import UniversalOptimizer
@@ -43,7 +44,7 @@ def __getattr__(name):
         from . import muon
 
         return getattr(muon, name)
-    if name in ("GradTable", "grad_norm", "clip_grad_norm_", "accumulate_grads_"):
+    if name in ("GradTable", "grad_norm", "clip_scale", "clip_grad_norm_", "accumulate_grads_"):
         from . import grads
 
         return getattr(grads, name)
@@ -52,4 +53,4 @@ def __getattr__(name):
 
 __all__ = ["Optimizer", "UniversalOptimizer", "AdamW", "Lion", "SGD", "Muon", "MuonND",
            "MultiDimensionalMuon", "zeropower_via_newtonschulz5", "GradTable", "grad_norm",
-           "clip_grad_norm_", "accumulate_grads_"]
+           "clip_scale", "clip_grad_norm_", "accumulate_grads_"]

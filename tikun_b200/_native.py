@@ -185,6 +185,8 @@ _SIGNATURES = {
     "tk_newton_schulz_2d": [_P, _I64, _I64, _I32, _I32, _I32, _P],
     "tk_newton_schulz_3d": [_P, _I64, _I64, _I64, _I32, _I32, _I32, _P],
     "tk_muon_step": [ctypes.POINTER(TkMuonLeaf), _SZ, ctypes.POINTER(TkMuonHParams), _P],
+    "tk_muon_step_clipped": [ctypes.POINTER(TkMuonLeaf), _SZ, ctypes.POINTER(TkMuonHParams), _P,
+                             _P],
     "tk_device_status": [ctypes.POINTER(ctypes.c_int)],
     "tk_testing_bounded_wait": [ctypes.c_int, _P],
     "tk_testing_gemm_tn": [_P, _P, _P, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
@@ -287,6 +289,18 @@ def step_fast_buffers_async(param_ptrs, grad_ptrs, m1_ptrs, m2_ptrs, lengths, ma
                                       current_stream() if stream is None else stream))
 
 
+def apply_pointwise(param_ptrs, grad_ptrs, m1_ptrs, m2_ptrs, lengths, opt_kind_name, step_count,
+                    lr, b1, b2, eps, decay, clip_scale_ptr: int, *, p_dtypes=None, g_dtypes=None,
+                    stream: int | None = None) -> None:
+    """The update of device leaves with the clip scale at ``clip_scale_ptr``
+    (device f32), formed elsewhere; does not wait."""
+    leaves, n = make_leaves(param_ptrs, grad_ptrs, m1_ptrs, m2_ptrs, lengths, p_dtypes, g_dtypes)
+    hp = TkHParams(lr, b1, b2, eps, decay)
+    check(lib().tk_apply_pointwise(leaves, n, opt_kind(opt_kind_name), ctypes.byref(hp),
+                                   int(step_count), clip_scale_ptr,
+                                   current_stream() if stream is None else stream))
+
+
 def newton_schulz_2d_ffi(matrix_ptr: int, rows: int, cols: int, steps: int, *,
                          dtype: int = TK_F32, precision: int | None = None,
                          stream: int | None = None) -> None:
@@ -307,9 +321,11 @@ def newton_schulz_3d_ffi(tensor_ptr: int, num_heads: int, head_dim_out: int, hea
 
 
 def muon_step(leaves: Sequence[tuple], lr: float, momentum: float, nesterov: bool = True,
-              ns_steps: int = 5, precision: int | None = None, stream: int | None = None) -> None:
+              ns_steps: int = 5, precision: int | None = None, stream: int | None = None,
+              clip_scale_ptr: int = 0) -> None:
     """Fused Muon update over (p_ptr, g_ptr, mom_ptr, heads, rows, cols, p_dtype,
-    g_dtype) leaves.  Device leaves: enqueued on the stream, does not wait.
+    g_dtype) leaves.  ``clip_scale_ptr`` (device f32): the gradients are
+    multiplied by it (device leaves only).  Device leaves: enqueued on the stream, does not wait.
     Host leaves (all of them; the reference's convention): streamed through
     device memory, returns when the results are back in host memory."""
     arr = (TkMuonLeaf * max(len(leaves), 1))()
@@ -317,8 +333,11 @@ def muon_step(leaves: Sequence[tuple], lr: float, momentum: float, nesterov: boo
         arr[i] = TkMuonLeaf(*L)
     hp = TkMuonHParams(lr, momentum, 1 if nesterov else 0, ns_steps,
                        DEFAULT_NS_PRECISION if precision is None else precision)
-    check(lib().tk_muon_step(arr, len(leaves), ctypes.byref(hp),
-                             current_stream() if stream is None else stream))
+    s = current_stream() if stream is None else stream
+    if clip_scale_ptr:
+        check(lib().tk_muon_step_clipped(arr, len(leaves), ctypes.byref(hp), clip_scale_ptr, s))
+    else:
+        check(lib().tk_muon_step(arr, len(leaves), ctypes.byref(hp), s))
 
 
 def device_status() -> int:

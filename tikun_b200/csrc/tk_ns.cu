@@ -1125,6 +1125,12 @@ __device__ __forceinline__ float muon_u(const PrepArgs& a, float& buf, float g) 
   return a.nesterov ? __fadd_rn(__fmul_rn(a.mu, buf), __fmul_rn(a.om, g)) : buf;
 }
 
+// The clip scale of the gradients, multiplied into each in f32 as the pointwise
+// step does; 1 without one (1 g = g).
+__device__ __forceinline__ float grad_scale(const PrepArgs& a) {
+  return a.g_scale != nullptr ? *a.g_scale : 1.0f;
+}
+
 // Pass 1: per matrix, optional Muon momentum update, f64 sum of squares of the
 // matrix handed to Newton-Schulz.  grid (nblk, batch); each block takes an
 // equal range of 4-element groups (128-bit momentum accesses).
@@ -1135,6 +1141,7 @@ prep_stats_kernel(const __grid_constant__ PrepArgs a, double* __restrict__ parti
   const int64_t total = a.m * a.n;
   const void* src = a.src[b];
   float* mom = MUON ? a.mom[b] : nullptr;
+  const float gs = MUON ? grad_scale(a) : 1.0f;
   const bool vec = ((uintptr_t)src % (SDT == TK_F32 ? 16 : 8)) == 0 &&
                    (!MUON || ((uintptr_t)mom % 16) == 0);
   const int64_t groups = vec ? total / 4 : 0;
@@ -1148,7 +1155,7 @@ prep_stats_kernel(const __grid_constant__ PrepArgs a, double* __restrict__ parti
       float4 m4 = *reinterpret_cast<float4*>(mom + q * 4);
       float bb[4] = {m4.x, m4.y, m4.z, m4.w};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) u[j] = muon_u(a, bb[j], g[j]);
+      for (int j = 0; j < 4; ++j) u[j] = muon_u(a, bb[j], __fmul_rn(g[j], gs));
       *reinterpret_cast<float4*>(mom + q * 4) = make_float4(bb[0], bb[1], bb[2], bb[3]);
     } else {
 #pragma unroll
@@ -1167,7 +1174,7 @@ prep_stats_kernel(const __grid_constant__ PrepArgs a, double* __restrict__ parti
     float u = g;
     if constexpr (MUON) {
       float bb = mom[i];
-      u = muon_u(a, bb, g);
+      u = muon_u(a, bb, __fmul_rn(g, gs));
       mom[i] = bb;
     }
     s = fma((double)u, (double)u, s);
@@ -1203,12 +1210,12 @@ prep_scale_kernel(const double* __restrict__ partials, int nblk, float* __restri
 // (python/tikun/muon_nd.py:112-115) or the input itself.
 template <int SDT, bool MUON>
 __device__ __forceinline__ float prep_value(const PrepArgs& a, const void* src, const float* mom,
-                                            int64_t i, float inv) {
+                                            int64_t i, float inv, float gs) {
   const float g = load_src1<SDT>(src, i);
   float u = g;
   if constexpr (MUON) {
     const float buf = mom[i];
-    u = a.nesterov ? __fadd_rn(__fmul_rn(a.mu, buf), __fmul_rn(a.om, g)) : buf;
+    u = a.nesterov ? __fadd_rn(__fmul_rn(a.mu, buf), __fmul_rn(a.om, __fmul_rn(g, gs))) : buf;
   }
   return __fmul_rn(u, inv);
 }
@@ -1229,13 +1236,14 @@ prep_output_kernel(const __grid_constant__ PrepArgs a, const float* __restrict__
   const float* mom = MUON ? a.mom[b] : nullptr;
   const int64_t c = tc * 32 + threadIdx.x;
   void* dst = a.dst[b];
+  const float gs = MUON ? grad_scale(a) : 1.0f;
   const float sc = tall ? a.upd_scale_tall : a.upd_scale_wide;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const int64_t r = tr * 32 + threadIdx.y + 8 * k;
     if (r >= rows || c >= cols) continue;
     const int64_t i = r * cols + c;
-    const float x = prep_value<SDT, MUON>(a, src, mom, i, inv);
+    const float x = prep_value<SDT, MUON>(a, src, mom, i, inv, gs);
     if (a.dst_dtype == TK_F32) {
       float* p = static_cast<float*>(dst) + i;
       *p = a.update ? __fadd_rn(*p, __fmul_rn(sc, x)) : x;
@@ -1271,6 +1279,7 @@ prep_write_kernel(const __grid_constant__ PrepArgs a, const float* __restrict__ 
   const int64_t r0 = (blockIdx.x / tiles_c) * T, c0 = (blockIdx.x % tiles_c) * T;
   const void* src = a.src[b];
   const float* mom = MUON ? a.mom[b] : nullptr;
+  const float gs = MUON ? grad_scale(a) : 1.0f;
   const int q = threadIdx.x & 15, y = threadIdx.x >> 4;
   // 4-element vector accesses of a row need every row start aligned
   const bool vec = (cols & 3) == 0 &&
@@ -1303,13 +1312,15 @@ prep_write_kernel(const __grid_constant__ PrepArgs a, const float* __restrict__ 
       for (int j = 0; j < 4; ++j) {
         float u = g[j];
         if constexpr (MUON)
-          u = a.nesterov ? __fadd_rn(__fmul_rn(a.mu, buf[j]), __fmul_rn(a.om, g[j])) : buf[j];
+          u = a.nesterov
+                  ? __fadd_rn(__fmul_rn(a.mu, buf[j]), __fmul_rn(a.om, __fmul_rn(g[j], gs)))
+                  : buf[j];
         x[j] = __fmul_rn(u, inv);
       }
     } else if (r < rows) {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (c + j < cols) x[j] = prep_value<SDT, MUON>(a, src, mom, r * cols + c + j, inv);
+        if (c + j < cols) x[j] = prep_value<SDT, MUON>(a, src, mom, r * cols + c + j, inv, gs);
     }
     uint16_t h[4], l[4];
 #pragma unroll
@@ -1602,6 +1613,7 @@ int run_group(const GroupLayout& L, const GroupIO& io, int steps, int fmt, void*
   pa.mu = io.mu;
   pa.om = io.om;
   pa.nesterov = io.nesterov;
+  pa.g_scale = io.g_scale;
   pa.xt = XT[0];
   pa.xt_ld = L.rsm;
   pa.xt_bs = L.n * L.rsm;

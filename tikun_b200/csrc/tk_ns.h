@@ -47,6 +47,7 @@ struct GroupIO {
   float mu, om;            // momentum and (1 - momentum) in f32
   int nesterov;
   const PeerSet* peers = nullptr;  // the final parameters also go to these peers
+  const float* g_scale = nullptr;  // device: the gradients are multiplied by it (Muon)
 };
 
 struct PrepArgs {
@@ -64,6 +65,7 @@ struct PrepArgs {
   int dst_dtype;
   int update;
   float upd_scale_wide, upd_scale_tall;
+  const float* g_scale;  // may be null
 };
 
 // Enqueues the whole iteration for one batch on stream s.  scratch holds

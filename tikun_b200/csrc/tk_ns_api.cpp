@@ -149,7 +149,7 @@ static int run_batches(int64_t m, int64_t n, const std::vector<const void*>& src
                        const std::vector<uint8_t>& tall, int src_dtype, int dst_dtype, int update,
                        float scale_wide, float scale_tall, float mu, float om, int nesterov,
                        int steps, int fmt, cudaStream_t s, const PeerSet* peers = nullptr,
-                       PeerCopy* copy = nullptr) {
+                       PeerCopy* copy = nullptr, const float* g_scale = nullptr) {
   const int64_t count = (int64_t)src.size();
   const ns::GroupLayout one = ns::group_layout(m, n, 1, fmt >= 2);
   int64_t per_wave = std::max<int64_t>(
@@ -180,6 +180,7 @@ static int run_batches(int64_t m, int64_t n, const std::vector<const void*>& src
     io.om = om;
     io.nesterov = nesterov;
     io.peers = peers;
+    io.g_scale = g_scale;
     TK_TRY(ns::run_group(L, io, steps, fmt, scratch.get(), status, s));
     if (copy != nullptr && copy->n > 0) {
       const size_t bytes = (size_t)m * (size_t)n * (dst_dtype == TK_F32 ? 4 : 2);
@@ -431,7 +432,8 @@ int tk_newton_schulz_3d(void* tensor, int64_t num_heads, int64_t head_dim_out,
 }
 
 static int muon_step(const tk_muon_leaf* leaves, size_t n_leaves, const tk_muon_hparams* hp,
-                     const PeerSet* peers, PeerCopy* copy, void* stream) {
+                     const PeerSet* peers, PeerCopy* copy, void* stream,
+                     const float* g_scale = nullptr) {
   if (hp == nullptr) return set_error(TK_ERR_INVALID, "hparams is NULL");
   if (n_leaves > 0 && leaves == nullptr) return set_error(TK_ERR_INVALID, "leaves is NULL");
   const int fmt = fmt_of(hp->precision);
@@ -514,6 +516,12 @@ static int muon_step(const tk_muon_leaf* leaves, size_t n_leaves, const tk_muon_
   }
   std::stable_sort(order.begin(), order.end(),
                    [](const auto& a, const auto& b) { return a.first < b.first; });
+  if (g_scale != nullptr) {
+    Residency r;
+    TK_TRY(classify_pointer(g_scale, &r, dev));
+    if (r != Residency::kDevice || where == Residency::kHost)
+      return set_error(TK_ERR_INVALID, "the clipped Muon step takes device buffers");
+  }
   if (where == Residency::kHost) {
     std::vector<HostGroup> hg;
     for (const auto& o : order) {
@@ -565,7 +573,7 @@ static int muon_step(const tk_muon_leaf* leaves, size_t n_leaves, const tk_muon_
     const float upd_tall = (float)(-hp->lr * std::sqrt(std::max(1.0, (double)n / (double)m)));
     TK_TRY(run_batches(m, n, kv.second.g, kv.second.p, &kv.second.mom, kv.second.tall, gdt, pdt,
                        1, upd_wide, upd_tall, mu, om, hp->nesterov ? 1 : 0, hp->ns_steps, fmt, gs,
-                       peers, copy));
+                       peers, copy, g_scale));
   }
   if (ks > 1)  // the caller's stream waits for every group
     for (int j = 0; j < ks; ++j) {
@@ -586,6 +594,13 @@ int tk_muon_step(const tk_muon_leaf* leaves, size_t n_leaves, const tk_muon_hpar
                  void* stream) {
   clear_error();
   return muon_step(leaves, n_leaves, hp, nullptr, nullptr, stream);
+}
+
+int tk_muon_step_clipped(const tk_muon_leaf* leaves, size_t n_leaves, const tk_muon_hparams* hp,
+                         const float* scale_dev, void* stream) {
+  clear_error();
+  if (scale_dev == nullptr) return set_error(TK_ERR_INVALID, "scale_dev is NULL");
+  return muon_step(leaves, n_leaves, hp, nullptr, nullptr, stream, scale_dev);
 }
 
 int tk_muon_step_peers(const tk_muon_leaf* leaves, size_t n_leaves, const tk_muon_hparams* hp,

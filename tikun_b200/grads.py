@@ -6,7 +6,8 @@ and fold the scale into their update, so that neither the norm nor a clipped
 gradient ever reaches memory.  The functions here are for programs that need
 those: a norm for the log (of the whole model, or of each tensor), clipped
 gradients for a consumer that does not clip, one norm over the gradients of
-several optimizers, or f32 sums of bf16 or f16 micro-batch gradients.
+several optimizers (``clip_scale``), or f32 sums of bf16 or f16 micro-batch
+gradients.
 
 Gradients are a PyTree (as ``UniversalOptimizer`` takes it) of CUDA tensors of
 one device, f32, bf16 or f16, in any mix and any number.  A ``Parameter``
@@ -219,6 +220,22 @@ def grad_norm(grads, norm_type: float = 2.0, per_tensor: bool = False,
     return (norm, each) if per_tensor else norm
 
 
+def clip_scale(grads, max_norm: float, norm_type: float = 2.0):
+    """(norm, scale): the norm of ``grad_norm`` and the scale that
+    ``clip_grad_norm_`` would multiply by, both 0-dim f32 tensors on the device.
+    The optimizers' ``step(clip_scale=scale)`` folds it into their updates, so
+    that several of them clip by one norm and no gradient is written."""
+    code = _norm_code(norm_type)
+    if not max_norm > 0:
+        raise ValueError(f"max_norm is positive, got {max_norm!r}")
+    t = _table(grads)
+    norm = torch.empty((), dtype=torch.float32, device=t.device)
+    scale = torch.empty((), dtype=torch.float32, device=t.device)
+    _on_device(t, lambda stream: _native.check(_native.lib().tk_grad_norm(
+        t._handle, code, max_norm, norm.data_ptr(), None, scale.data_ptr(), stream)))
+    return norm, scale
+
+
 def clip_grad_norm_(grads, max_norm: float, norm_type: float = 2.0, out=None,
                     error_if_nonfinite: bool = False) -> torch.Tensor:
     """Scales the gradients by ``max_norm / (norm + 1e-6)`` if their norm (see
@@ -265,4 +282,4 @@ def accumulate_grads_(grads, acc=None, alpha: float = 1.0, overwrite: bool = Fal
     return norm
 
 
-__all__ = ["GradTable", "grad_norm", "clip_grad_norm_", "accumulate_grads_"]
+__all__ = ["GradTable", "grad_norm", "clip_scale", "clip_grad_norm_", "accumulate_grads_"]

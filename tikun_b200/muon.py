@@ -16,8 +16,9 @@ from __future__ import annotations
 import torch
 
 from . import _native
+from .grads import clip_scale as scale_of
 from .muon_nd import MultiDimensionalMuon
-from .universal import UniversalOptimizer, _tk_dtype
+from .universal import UniversalOptimizer, _tk_dtype, check_clip_scale
 
 
 def zeropower_via_newtonschulz5(G: torch.Tensor, steps: int = 5, eps: float = 1e-7,
@@ -37,11 +38,16 @@ def zeropower_via_newtonschulz5(G: torch.Tensor, steps: int = 5, eps: float = 1e
 class Muon(torch.optim.Optimizer):
     def __init__(self, muon_params, adamw_params=None, lr: float = 0.02, momentum: float = 0.95,
                  adamw_lr: float = 6e-4, adamw_betas: tuple = (0.9, 0.95), adamw_decay: float = 0.1,
-                 precision: int | None = None):
+                 precision: int | None = None, max_norm: float = 0.0):
+        """``max_norm`` > 0 clips all gradients, ``muon_params``' and
+        ``adamw_params``', by their common L2 norm (see ``MultiDimensionalMuon``)."""
         muon_params = list(muon_params)
         super().__init__(muon_params, dict(lr=lr, momentum=momentum))
         self.lr = lr
         self.momentum = momentum
+        self.max_norm = max_norm
+        self.grad_norm = None
+        self.clip_scale = None
         self.step_count = 0
         self.precision = _native.DEFAULT_NS_PRECISION if precision is None else precision
         self.state_momentum = [torch.zeros(p.shape, dtype=torch.float32, device=p.device)
@@ -55,8 +61,14 @@ class Muon(torch.optim.Optimizer):
                                                 weight_decay=adamw_decay)
 
     @torch.no_grad()
-    def step(self):
-        """muon.py:79-102."""
+    def step(self, clip_scale=None):
+        """muon.py:79-102.  ``clip_scale``: see ``MultiDimensionalMuon.step``."""
+        if clip_scale is not None:
+            check_clip_scale(clip_scale, self.max_norm)
+        elif self.max_norm > 0:
+            params = self.param_groups[0]["params"] + (self.adamw.params if self.adamw else [])
+            self.grad_norm, clip_scale = scale_of([p.grad for p in params], self.max_norm)
+        self.clip_scale = clip_scale
         self.step_count += 1
         leaves = []
         for i, p in enumerate(self.param_groups[0]["params"]):
@@ -70,9 +82,10 @@ class Muon(torch.optim.Optimizer):
                            p.shape[1], _tk_dtype(p), _tk_dtype(p.grad)))
         if leaves:
             _native.muon_step(leaves, self.lr, self.momentum, nesterov=False, ns_steps=5,
-                              precision=self.precision)
+                              precision=self.precision,
+                              clip_scale_ptr=0 if clip_scale is None else clip_scale.data_ptr())
         if self.adamw is not None:
-            self.adamw.step()
+            self.adamw.step(clip_scale=clip_scale)
 
 
 __all__ = ["Muon", "MultiDimensionalMuon", "zeropower_via_newtonschulz5"]

@@ -21,6 +21,12 @@ few strong directions over a noise floor stays within 1.5e-3 of f32, at 1.4
 to 1.5 times the f16 time) or ``TK_NS_F16X3`` (all operands as f16 pairs:
 within a few 1e-6, for bf16 parameters held to 1e-3 over many steps, at 3
 times).
+
+``max_norm`` > 0 clips all gradients, those of the Newton-Schulz leaves and of
+the AdamW leaves, by their common L2 norm, as the pointwise optimizers clip by
+theirs: the scale is folded into both updates, the gradients stay as they are,
+and ``grad_norm`` and ``clip_scale`` hold the last step's values on the device.
+(The reference's Muon does not clip.)
 """
 from __future__ import annotations
 
@@ -29,7 +35,8 @@ import math
 import numpy as np
 
 from . import _native
-from .universal import UniversalOptimizer, _extract_pointer_and_len, _flatten_pytree, _tk_dtype
+from .universal import (UniversalOptimizer, _extract_pointer_and_len, _flatten_pytree, _tk_dtype,
+                        check_clip_scale)
 
 
 def _ndim(p) -> int:
@@ -39,7 +46,7 @@ def _ndim(p) -> int:
 class MultiDimensionalMuon:
     def __init__(self, params, lr: float = 0.02, momentum: float = 0.95, nesterov: bool = True,
                  ns_steps: int = 5, adamw_lr: float = 1e-3, adamw_betas: tuple = (0.9, 0.999),
-                 adamw_decay: float = 0.01, precision: int | None = None):
+                 adamw_decay: float = 0.01, precision: int | None = None, max_norm: float = 0.0):
         self.raw_params = _flatten_pytree(params)
         self.lr = lr
         self.momentum = momentum
@@ -49,6 +56,9 @@ class MultiDimensionalMuon:
         self.adamw_b1, self.adamw_b2 = adamw_betas
         self.adamw_decay = adamw_decay
         self.precision = _native.DEFAULT_NS_PRECISION if precision is None else precision
+        self.max_norm = max_norm
+        self.grad_norm = None
+        self.clip_scale = None
         self.step_count = 0
         self.rank_1_params, self.rank_2_params, self.rank_nd_params = [], [], []
         self.momentum_state = {}
@@ -87,19 +97,30 @@ class MultiDimensionalMuon:
         return (p_ptr, g.data_ptr(), mom.data_ptr(), heads, shape[-2], shape[-1], _tk_dtype(p),
                 _tk_dtype(g))
 
-    def step(self):
-        """muon_nd.py:94-160."""
+    def step(self, clip_scale=None):
+        """muon_nd.py:94-160.  ``clip_scale`` (a 0-dim f32 CUDA tensor, as
+        ``grads.clip_scale`` returns it): the scale of a norm over more gradients
+        than this optimizer's."""
+        if clip_scale is not None:
+            check_clip_scale(clip_scale, self.max_norm)
+        elif self.max_norm > 0:
+            from .grads import clip_scale as scale_of
+
+            self.grad_norm, clip_scale = scale_of(
+                [getattr(p, "grad", None) for p in self.raw_params], self.max_norm)
+        self.clip_scale = clip_scale
         self.step_count += 1
         # 1. 1-D leaves: AdamW (eps 1e-8, no clip) with this optimizer's step count
         if self.rank_1_params:
             self._adamw.step_count = self.step_count - 1
-            self._adamw.step()
+            self._adamw.step(clip_scale=clip_scale)
         # 2./3. 2-D and N-D leaves: one fused Muon call
         leaves = [self._muon_leaf(p) for p in self.rank_2_params + self.rank_nd_params
                   if getattr(p, "grad", None) is not None]
         if leaves:
             _native.muon_step(leaves, self.lr, self.momentum, self.nesterov, self.ns_steps,
-                              self.precision)
+                              self.precision,
+                              clip_scale_ptr=0 if clip_scale is None else clip_scale.data_ptr())
 
 
 def update_scale(rows: int, cols: int) -> float:

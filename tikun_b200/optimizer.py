@@ -23,7 +23,7 @@ from __future__ import annotations
 import torch
 
 from . import _native
-from .universal import leaf_address
+from .universal import check_clip_scale, leaf_address
 
 
 class AdamW(torch.optim.Optimizer):
@@ -64,7 +64,11 @@ class AdamW(torch.optim.Optimizer):
         return st["m1"], st["m2"]
 
     @torch.no_grad()
-    def step(self, closure=None):
+    def step(self, closure=None, clip_scale=None):
+        """``clip_scale`` (a 0-dim f32 CUDA tensor, as ``grads.clip_scale``
+        returns it) takes the place of this optimizer's own norm."""
+        if clip_scale is not None:
+            check_clip_scale(clip_scale, self.param_groups[0]["max_norm"])
         loss = None
         if closure is not None:
             with torch.enable_grad():
@@ -93,7 +97,15 @@ class AdamW(torch.optim.Optimizer):
                 self.step_count, group["lr"], group["beta_one"], group["beta_two"], group["eps"],
                 group["weight_decay"])
         devices = {p.device for p in params}
-        if len(devices) == 1 and params[0].is_cuda:
+        if clip_scale is not None:
+            if devices != {clip_scale.device}:
+                raise ValueError("clip_scale is on the device of the parameters, got "
+                                 f"{clip_scale.device}")
+            with torch.cuda.device(clip_scale.device):
+                _native.apply_pointwise(*args[:5], *args[6:], clip_scale.data_ptr(),
+                                        p_dtypes=p_dt, g_dtypes=g_dt)
+            self.clip_scale = clip_scale
+        elif len(devices) == 1 and params[0].is_cuda:
             dev = params[0].device
             if self.clip_scale is None or not isinstance(self.clip_scale, torch.Tensor) or \
                     self.clip_scale.device != dev:

@@ -111,6 +111,16 @@ def _is_cuda(t) -> bool:
     return bool(getattr(t, "is_cuda", False))
 
 
+def check_clip_scale(scale, max_norm: float, in_backward: bool = False) -> None:
+    """Refuses a clip scale that a step cannot use."""
+    if not _is_cuda(scale) or str(scale.dtype) != "torch.float32" or scale.numel() != 1:
+        raise ValueError("clip_scale is one float32 value on a CUDA device")
+    if max_norm > 0:
+        raise ValueError("an optimizer with max_norm forms its own clip scale")
+    if in_backward:
+        raise ValueError("in_backward steps each leaf before a common norm is known")
+
+
 class UniversalOptimizer:
     """See the module docstring; arguments as python/tikun/universal.py:67-78."""
 
@@ -161,8 +171,20 @@ class UniversalOptimizer:
         return _extract_pointer_and_len(m1)[0], _extract_pointer_and_len(m2)[0]
 
     def _call(self, p_ptrs, g_ptrs, m1_ptrs, m2_ptrs, lengths, p_dt, g_dt, step, on_device,
-              device=None):
-        if on_device:
+              device=None, clip_scale=None):
+        if clip_scale is not None:
+            if not on_device or clip_scale.device != device:
+                raise ValueError("clip_scale is on the device of the parameters, got "
+                                 f"{clip_scale.device}")
+            import torch
+
+            with torch.cuda.device(device):
+                _native.apply_pointwise(
+                    p_ptrs, g_ptrs, m1_ptrs, m2_ptrs, lengths, self.algorithm, step, self.lr,
+                    self.beta1, self.beta2, self.eps, self.weight_decay, clip_scale.data_ptr(),
+                    p_dtypes=p_dt, g_dtypes=g_dt)
+            self.clip_scale = clip_scale
+        elif on_device:
             import torch
 
             if self.clip_scale is None or self.clip_scale.device != device:
@@ -199,13 +221,17 @@ class UniversalOptimizer:
                    max(1, self.step_count), _is_cuda(p), getattr(p, "device", None))
 
     # -- step ----------------------------------------------------------------
-    def step(self, grads=None):
-        """universal.py:139-192."""
+    def step(self, grads=None, clip_scale=None):
+        """universal.py:139-192.  ``clip_scale`` (a 0-dim f32 CUDA tensor, as
+        ``grads.clip_scale`` returns it) takes the place of this optimizer's own
+        norm: for a clip over more gradients than its own."""
+        if clip_scale is not None:
+            check_clip_scale(clip_scale, self.max_norm, self.in_backward)
         self.step_count += 1
         if self.in_backward:
             return
         if self._arena is not None:
-            self._arena.step(self, grads)
+            self._arena.step(self, grads, clip_scale)
             return
         p_ptrs, g_ptrs, m1_ptrs, m2_ptrs, lengths, p_dt, g_dt = [], [], [], [], [], [], []
         flat_grads = _flatten_pytree(grads) if grads is not None else None
@@ -235,7 +261,7 @@ class UniversalOptimizer:
             return
         on_device = all(cuda_flags)
         self._call(p_ptrs, g_ptrs, m1_ptrs, m2_ptrs, lengths, p_dt, g_dt, self.step_count,
-                   on_device, device)
+                   on_device, device, clip_scale)
 
     def zero_grad(self):
         if self._arena is not None:  # the gradients stay views of the arena
@@ -351,7 +377,7 @@ class _ArenaState:
     def moments(self):
         return [(self.m1.leaf(i), self.m2.leaf(i)) for i in range(self.n_params)]
 
-    def step(self, opt, grads=None):
+    def step(self, opt, grads=None, clip_scale=None):
         import ctypes
 
         import torch
@@ -364,6 +390,17 @@ class _ArenaState:
                 for i, g in enumerate(flat):
                     self.grads.leaf(i).copy_(torch.as_tensor(g, device=self.device).reshape(-1))
         hp = _native.TkHParams(opt.lr, opt.beta1, opt.beta2, opt.eps, opt.weight_decay)
+        if clip_scale is not None:
+            if clip_scale.device != self.device:
+                raise ValueError("clip_scale is on the device of the parameters, got "
+                                 f"{clip_scale.device}")
+            with torch.cuda.device(self.device):
+                _native.check(_native.lib().tk_apply_pointwise(
+                    self.leaves, self.n, _native.opt_kind(opt.algorithm), ctypes.byref(hp),
+                    opt.step_count, clip_scale.data_ptr(),
+                    torch.cuda.current_stream().cuda_stream))
+            opt.clip_scale = clip_scale
+            return
         with torch.cuda.device(self.device):
             _native.check(_native.lib().tk_step_buffers_async(
                 self.leaves, self.n, _native.opt_kind(opt.algorithm), ctypes.byref(hp),
