@@ -39,16 +39,15 @@ def SGD(params, lr=1e-2, momentum=0.9, weight_decay=0.0, max_norm=0.0, in_backwa
 
 
 def __getattr__(name):
-    # these import torch: only when one is asked for
+    # these import torch: only when one is asked for, and then kept
     if name in ("Muon", "zeropower_via_newtonschulz5"):
-        from . import muon
-
-        return getattr(muon, name)
-    if name in ("GradTable", "grad_norm", "clip_scale", "clip_grad_norm_", "accumulate_grads_"):
-        from . import grads
-
-        return getattr(grads, name)
-    raise AttributeError(name)
+        from . import muon as module
+    elif name in ("GradTable", "grad_norm", "clip_scale", "clip_grad_norm_", "accumulate_grads_"):
+        from . import grads as module
+    else:
+        raise AttributeError(name)
+    value = globals()[name] = getattr(module, name)
+    return value
 
 
 __all__ = ["Optimizer", "UniversalOptimizer", "AdamW", "Lion", "SGD", "Muon", "MuonND",

@@ -76,7 +76,8 @@ inline uint64_t tiles_of(int g_dtype, uint64_t phase, uint64_t n) {
 }
 
 // Sum of powers (or largest magnitude) of each tile into partials[0..p.tiles).
-int launch_norm(const GradPart& p, int norm, double* partials, cudaStream_t s);
+// again: launch_clip will read the tiles once more, the last ones first.
+int launch_norm(const GradPart& p, int norm, bool again, double* partials, cudaStream_t s);
 // out = out + alpha g, or alpha g, and the same of each tile of the new out;
 // norm TK_NORM_NONE: without it.
 int launch_sum(const GradPart& p, int norm, float alpha, bool overwrite, double* partials,

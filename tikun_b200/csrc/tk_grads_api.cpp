@@ -160,9 +160,9 @@ size_t tiles_of(const tk_grad_table& t) {
 }
 
 // Every part's partials, one after the other.
-int norm_parts(const tk_grad_table& t, int norm, double* partials, cudaStream_t s) {
+int norm_parts(const tk_grad_table& t, int norm, bool again, double* partials, cudaStream_t s) {
   for (const auto& p : t.parts) {
-    if (p.tiles) TK_TRY(gr::launch_norm(p, norm, partials, s));
+    if (p.tiles) TK_TRY(gr::launch_norm(p, norm, again, partials, s));
     partials += p.tiles;
   }
   return TK_OK;
@@ -179,7 +179,7 @@ int grad_norm(const tk_grad_table& t, int norm, const gr::NormOut& out, float* e
   Scratch sc;
   TK_TRY(sc.alloc(sizeof(double) * total, s));
   double* partials = static_cast<double*>(sc.get());
-  TK_TRY(norm_parts(t, norm, partials, s));
+  TK_TRY(norm_parts(t, norm, false, partials, s));
   if (each_dev == nullptr || t.parts.empty())
     return gr::launch_fold(norm, partials, (int64_t)total, out, s);
   const double* at = partials;
@@ -199,7 +199,7 @@ int clip_grad_norm(const tk_grad_table& t, int norm, gr::NormOut out, cudaStream
   TK_TRY(sc.alloc(sizeof(double) * (total + 1), s));
   double* partials = static_cast<double*>(sc.get());
   out.scale_too = reinterpret_cast<float*>(partials + total);
-  TK_TRY(norm_parts(t, norm, partials, s));
+  TK_TRY(norm_parts(t, norm, true, partials, s));
   TK_TRY(gr::launch_fold(norm, partials, (int64_t)total, out, s));
   for (size_t i = t.parts.size(); i-- > 0;)  // the norm's last part first
     if (t.parts[i].tiles) TK_TRY(gr::launch_clip(t.parts[i], out.scale_too, s));

@@ -128,6 +128,7 @@ class GradTable:
 
     def __init__(self, grads, out=None):
         self._handle = None
+        self._like = None
         self._params = []
         self.grads = _leaves(grads)
         # a plain tensor is no Parameter (whose isinstance costs ten times as much)
@@ -177,6 +178,13 @@ class GradTable:
             self._destroy(self._handle)
             self._handle = None
 
+    def _result(self) -> torch.Tensor:
+        """A 0-dim f32 tensor for a call's result."""
+        if self._like is None:
+            self._like = torch.empty((), dtype=torch.float32, device=self.device)
+            return self._like
+        return torch.empty_like(self._like)  # a microsecond less
+
     def _standing(self) -> "GradTable":
         for p, g in self._params:
             if p.grad is not g:
@@ -210,7 +218,7 @@ def grad_norm(grads, norm_type: float = 2.0, per_tensor: bool = False,
     gradients, one each."""
     code = _norm_code(norm_type)
     t = _table(grads)
-    norm = torch.empty((), dtype=torch.float32, device=t.device)
+    norm = t._result()
     each = torch.empty(len(t), dtype=torch.float32, device=t.device) if per_tensor else None
     each_ptr = each.data_ptr() if per_tensor and len(t) else None
     _on_device(t, lambda stream: _native.check(_native.lib().tk_grad_norm(
@@ -229,8 +237,8 @@ def clip_scale(grads, max_norm: float, norm_type: float = 2.0):
     if not max_norm > 0:
         raise ValueError(f"max_norm is positive, got {max_norm!r}")
     t = _table(grads)
-    norm = torch.empty((), dtype=torch.float32, device=t.device)
-    scale = torch.empty((), dtype=torch.float32, device=t.device)
+    norm = t._result()
+    scale = t._result()
     _on_device(t, lambda stream: _native.check(_native.lib().tk_grad_norm(
         t._handle, code, max_norm, norm.data_ptr(), None, scale.data_ptr(), stream)))
     return norm, scale
@@ -255,7 +263,7 @@ def clip_grad_norm_(grads, max_norm: float, norm_type: float = 2.0, out=None,
     t = _table(grads, out)
     if error_if_nonfinite:
         grad_norm(t, norm_type, error_if_nonfinite=True)
-    norm = torch.empty((), dtype=torch.float32, device=t.device)
+    norm = t._result()
     _on_device(t, lambda stream: _native.check(_native.lib().tk_clip_grad_norm(
         t._handle, code, max_norm, norm.data_ptr(), None, stream)))
     return norm
@@ -275,7 +283,7 @@ def accumulate_grads_(grads, acc=None, alpha: float = 1.0, overwrite: bool = Fal
     if not isinstance(grads, GradTable) and acc is None:
         raise ValueError("accumulate_grads_ needs acc")
     t = _table(grads, acc)
-    norm = torch.empty((), dtype=torch.float32, device=t.device) if norm_type is not None else None
+    norm = t._result() if norm_type is not None else None
     norm_ptr = norm.data_ptr() if norm is not None else None
     _on_device(t, lambda stream: _native.check(_native.lib().tk_accumulate_grads(
         t._handle, alpha, 1 if overwrite else 0, code, norm_ptr, stream)))
