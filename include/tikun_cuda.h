@@ -244,6 +244,13 @@ typedef struct tk_grad_table tk_grad_table;
 TK_API int tk_grad_table_create(const tk_grad* grads, size_t n, tk_grad_table** out);
 TK_API int tk_grad_table_destroy(tk_grad_table* table);
 
+/* Scratch that a call on the table needs: *bytes, and *bytes_each for
+ * tk_grad_norm with each_dev (0: none).  A call takes it at `workspace` (device
+ * memory, 8-byte aligned, written and read by that call's kernels only, so that
+ * calls whose kernels may overlap need one each), or with NULL from the
+ * library's own stream-ordered pool, which costs the stream about 2 us. */
+TK_API int tk_grad_workspace(const tk_grad_table* table, uint64_t* bytes, uint64_t* bytes_each);
+
 /* TK_NORM_L2 sqrt(sum x^2), TK_NORM_L1 sum |x|, TK_NORM_MAX max |x|: over all
  * elements of all tensors, 0 for none.  A NaN element makes each of them NaN.
  * The sums are formed in a fixed order, so equal inputs give equal bits. */
@@ -255,21 +262,21 @@ enum { TK_NORM_NONE = -1, TK_NORM_L2 = 0, TK_NORM_L1 = 1, TK_NORM_MAX = 2 };
  * NaN).  All three are device memory and each may be NULL.  Stream-ordered;
  * does not wait. */
 TK_API int tk_grad_norm(const tk_grad_table* table, int32_t norm, float max_norm, float* norm_dev,
-                        float* each_dev, float* scale_dev, void* stream);
+                        float* each_dev, float* scale_dev, void* workspace, void* stream);
 
 /* out = scale * g, the product formed in f32 and rounded once to out's type,
  * with the scale of tk_grad_norm; max_norm > 0.  A tensor in place is left as
  * it is when the scale is 1.  TK_ERR_INVALID if a tensor in place shares
  * memory with another buffer of the table. */
 TK_API int tk_clip_grad_norm(const tk_grad_table* table, int32_t norm, float max_norm,
-                             float* norm_dev, float* scale_dev, void* stream);
+                             float* norm_dev, float* scale_dev, void* workspace, void* stream);
 
 /* out = out + alpha * g (one f32 rounding), or with overwrite out = alpha * g,
  * for out buffers of TK_F32 that are not in place.  With norm other than
  * TK_NORM_NONE, the norm of the new out to *norm_dev, formed in the same
  * pass. */
 TK_API int tk_accumulate_grads(const tk_grad_table* table, float alpha, int32_t overwrite,
-                               int32_t norm, float* norm_dev, void* stream);
+                               int32_t norm, float* norm_dev, void* workspace, void* stream);
 
 /* ---------------------------------------------------------------------- */
 /* Newton-Schulz (Muon)                                                    */

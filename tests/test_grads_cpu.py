@@ -48,9 +48,10 @@ def test_null_arguments():
     assert L.tk_grad_table_create(None, 0, None) == _native.TK_ERR_INVALID
     assert L.tk_grad_table_create(None, 3, ctypes.byref(h)) == _native.TK_ERR_INVALID
     assert L.tk_grad_table_destroy(None) == 0
-    for st in (L.tk_grad_norm(None, 0, 0.0, None, None, None, None),
-               L.tk_clip_grad_norm(None, 0, 1.0, None, None, None),
-               L.tk_accumulate_grads(None, 1.0, 0, -1, None, None)):
+    assert L.tk_grad_workspace(None, None, None) == _native.TK_ERR_INVALID
+    for st in (L.tk_grad_norm(None, 0, 0.0, None, None, None, None, None),
+               L.tk_clip_grad_norm(None, 0, 1.0, None, None, None, None),
+               L.tk_accumulate_grads(None, 1.0, 0, -1, None, None, None)):
         assert st == _native.TK_ERR_INVALID and b"null gradient table" in L.tk_last_error()
 
 

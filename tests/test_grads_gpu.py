@@ -302,6 +302,59 @@ def test_refusals_with_device_tensors():
         _native.check(_native.lib().tk_grad_table_create(arr, 1, ctypes.byref(h)))
 
 
+@pytest.mark.parametrize("sizes", [[4097], [1_000_003, 5, 300_000]], ids=["small", "large"])
+def test_workspace_of_the_caller_or_the_pool(sizes):
+    """The C calls give the same bits with either, write nothing behind the
+    bytes they ask for, and refuse what is not device memory."""
+    L = _native.lib()
+    ts = tensors(sizes, torch.bfloat16)
+    acc = [torch.zeros(n, device="cuda") for n in sizes]
+    t = GradTable(ts, out=acc)
+    b, be = ctypes.c_uint64(), ctypes.c_uint64()
+    _native.check(L.tk_grad_workspace(t._handle, ctypes.byref(b), ctypes.byref(be)))
+    assert (b.value == 0) == (len(sizes) == 1) and be.value > 0 and be.value % 8 == 0
+    s = torch.cuda.current_stream().cuda_stream
+    got = []
+    for with_ws in (False, True):
+        res = torch.zeros(4 + len(sizes), device="cuda")
+        at = [res[i:].data_ptr() for i in range(5)]
+        ws = torch.full((be.value // 8 + 8,), 7.0, dtype=torch.float64, device="cuda")
+        w = ws.data_ptr() if with_ws else None
+        _native.check(L.tk_grad_norm(t._handle, 0, 0.5, at[0], at[4], at[1], w, s))
+        _native.check(L.tk_clip_grad_norm(t._handle, 1, 0.5, at[2], None, w, s))
+        clipped = [a.clone() for a in acc]
+        _native.check(L.tk_accumulate_grads(t._handle, 0.5, 1, 2, at[3], w, s))
+        assert (ws[be.value // 8:] == 7.0).all()
+        got.append([res] + clipped + [a.clone() for a in acc])
+    for x, y in zip(*got):
+        assert same_bits(x, y)
+    host = torch.zeros(8, dtype=torch.float64)
+    pinned = torch.zeros(8, dtype=torch.float64).pin_memory()
+    dev = torch.zeros(8, dtype=torch.float64, device="cuda")
+    for bad in (host.data_ptr(), pinned.data_ptr(), dev.data_ptr() + 4):
+        with pytest.raises(ValueError, match="for a workspace"):
+            _native.check(L.tk_grad_norm(t._handle, 0, 0.0, dev.data_ptr(), None, None, bad, s))
+    for bad in (host.data_ptr(), pinned.data_ptr(), dev.data_ptr() + 2):
+        for args in ((bad, None, None), (None, bad, None), (None, None, bad)):
+            with pytest.raises(ValueError, match="for a result"):
+                _native.check(L.tk_grad_norm(t._handle, 0, 0.0, *args, None, s))
+        with pytest.raises(ValueError, match="for a result"):
+            _native.check(L.tk_clip_grad_norm(t._handle, 0, 1.0, bad, None, None, s))
+        with pytest.raises(ValueError, match="for a result"):
+            _native.check(L.tk_accumulate_grads(t._handle, 1.0, 1, 0, bad, None, s))
+    with pytest.raises(ValueError, match="norm_dev is NULL"):
+        _native.check(L.tk_accumulate_grads(t._handle, 1.0, 1, 0, None, None, s))
+    for call in (lambda: L.tk_grad_norm(t._handle, 3, 0.0, None, None, None, None, s),
+                 lambda: L.tk_grad_norm(t._handle, -1, 0.0, None, None, None, None, s),
+                 lambda: L.tk_clip_grad_norm(t._handle, 7, 1.0, None, None, None, s),
+                 lambda: L.tk_accumulate_grads(t._handle, 1.0, 1, 5, None, None, s)):
+        with pytest.raises(ValueError, match="unknown norm"):
+            _native.check(call())
+    for bad in (0.0, -1.0, math.nan):
+        with pytest.raises(ValueError, match="is not positive"):
+            _native.check(L.tk_clip_grad_norm(t._handle, 0, bad, None, None, None, s))
+
+
 def test_parameters_stand_for_their_gradients():
     lin = torch.nn.Linear(33, 17, device="cuda")
     frozen = torch.nn.Parameter(torch.zeros(5, device="cuda"))

@@ -179,9 +179,10 @@ _SIGNATURES = {
                                 _U64, _F, ctypes.POINTER(_F), _P],
     "tk_grad_table_create": [ctypes.POINTER(TkGrad), _SZ, ctypes.POINTER(_P)],
     "tk_grad_table_destroy": [_P],
-    "tk_grad_norm": [_P, _I32, _F, _P, _P, _P, _P],
-    "tk_clip_grad_norm": [_P, _I32, _F, _P, _P, _P],
-    "tk_accumulate_grads": [_P, _F, _I32, _I32, _P, _P],
+    "tk_grad_workspace": [_P, ctypes.POINTER(_U64), ctypes.POINTER(_U64)],
+    "tk_grad_norm": [_P, _I32, _F, _P, _P, _P, _P, _P],
+    "tk_clip_grad_norm": [_P, _I32, _F, _P, _P, _P, _P],
+    "tk_accumulate_grads": [_P, _F, _I32, _I32, _P, _P, _P],
     "tk_newton_schulz_2d": [_P, _I64, _I64, _I32, _I32, _I32, _P],
     "tk_newton_schulz_3d": [_P, _I64, _I64, _I64, _I32, _I32, _I32, _P],
     "tk_muon_step": [ctypes.POINTER(TkMuonLeaf), _SZ, ctypes.POINTER(TkMuonHParams), _P],

@@ -3,6 +3,7 @@
 #include <cuda_runtime.h>
 
 #include <exception>
+#include <initializer_list>
 #include <memory>
 #include <vector>
 
@@ -168,17 +169,27 @@ int norm_parts(const tk_grad_table& t, int norm, bool again, double* partials, c
   return TK_OK;
 }
 
+// The caller's workspace, or `count` f64 of the pool's.
+int scratch(void* workspace, size_t count, Scratch* pool, cudaStream_t s, double** out) {
+  if (workspace == nullptr) {
+    TK_TRY(pool->alloc(sizeof(double) * count, s));
+    workspace = pool->get();
+  }
+  *out = static_cast<double*>(workspace);
+  return TK_OK;
+}
+
 bool small(const tk_grad_table& t) { return t.parts.size() == 1 && gr::small(t.parts[0]); }
 
 int grad_norm(const tk_grad_table& t, int norm, const gr::NormOut& out, float* each_dev,
-              cudaStream_t s) {
+              void* workspace, cudaStream_t s) {
   NvtxRange r("tikun/grad_norm");
   if (each_dev == nullptr && small(t))
     return gr::launch_small(t.parts[0], gr::SMALL_NORM, norm, 0.0f, out, s);
   const size_t total = tiles_of(t);
-  Scratch sc;
-  TK_TRY(sc.alloc(sizeof(double) * total, s));
-  double* partials = static_cast<double*>(sc.get());
+  Scratch pool;
+  double* partials = nullptr;
+  TK_TRY(scratch(workspace, total, &pool, s, &partials));
   TK_TRY(norm_parts(t, norm, false, partials, s));
   if (each_dev == nullptr || t.parts.empty())
     return gr::launch_fold(norm, partials, (int64_t)total, out, s);
@@ -191,13 +202,14 @@ int grad_norm(const tk_grad_table& t, int norm, const gr::NormOut& out, float* e
   return TK_OK;
 }
 
-int clip_grad_norm(const tk_grad_table& t, int norm, gr::NormOut out, cudaStream_t s) {
+int clip_grad_norm(const tk_grad_table& t, int norm, gr::NormOut out, void* workspace,
+                   cudaStream_t s) {
   NvtxRange r("tikun/clip_grad_norm");
   if (small(t)) return gr::launch_small(t.parts[0], gr::SMALL_CLIP, norm, 0.0f, out, s);
   const size_t total = tiles_of(t);
-  Scratch sc;
-  TK_TRY(sc.alloc(sizeof(double) * (total + 1), s));
-  double* partials = static_cast<double*>(sc.get());
+  Scratch pool;
+  double* partials = nullptr;
+  TK_TRY(scratch(workspace, total + 1, &pool, s, &partials));
   out.scale_too = reinterpret_cast<float*>(partials + total);
   TK_TRY(norm_parts(t, norm, true, partials, s));
   TK_TRY(gr::launch_fold(norm, partials, (int64_t)total, out, s));
@@ -207,7 +219,7 @@ int clip_grad_norm(const tk_grad_table& t, int norm, gr::NormOut out, cudaStream
 }
 
 int accumulate(const tk_grad_table& t, float alpha, bool overwrite, int norm, float* norm_dev,
-               cudaStream_t s) {
+               void* workspace, cudaStream_t s) {
   NvtxRange r("tikun/accumulate_grads");
   gr::NormOut out;
   out.norm = norm_dev;
@@ -216,18 +228,33 @@ int accumulate(const tk_grad_table& t, float alpha, bool overwrite, int norm, fl
     return gr::launch_small(t.parts[0], overwrite ? gr::SMALL_FIRST : gr::SMALL_SUM, norm, alpha,
                             out, s);
   const size_t total = tiles_of(t);
-  Scratch sc;
+  Scratch pool;
   double* partials = nullptr;
-  if (with) {
-    TK_TRY(sc.alloc(sizeof(double) * total, s));
-    partials = static_cast<double*>(sc.get());
-  }
+  if (with) TK_TRY(scratch(workspace, total, &pool, s, &partials));
   double* at = partials;
   for (const auto& p : t.parts) {
     if (p.tiles) TK_TRY(gr::launch_sum(p, norm, alpha, overwrite, at, s));
     if (with) at += p.tiles;
   }
   return with ? gr::launch_fold(norm, partials, (int64_t)total, out, s) : TK_OK;
+}
+
+// A call's own device buffers, each of which may be null.
+int check_outputs(const tk_grad_table* t, std::initializer_list<const void*> four_byte,
+                  const void* workspace) {
+  for (const void* p : four_byte) {
+    if (p == nullptr) continue;
+    Residency r;
+    TK_TRY(classify_pointer(p, &r, t->dev));
+    if (r != Residency::kDevice || (uintptr_t)p % 4 != 0)
+      return set_error(TK_ERR_INVALID, "%p is not aligned device memory for a result", p);
+  }
+  if (workspace == nullptr) return TK_OK;
+  Residency r;
+  TK_TRY(classify_pointer(workspace, &r, t->dev));
+  if (r != Residency::kDevice || (uintptr_t)workspace % 8 != 0)
+    return set_error(TK_ERR_INVALID, "%p is not aligned device memory for a workspace", workspace);
+  return TK_OK;
 }
 
 // No C++ exception leaves a C entry point.
@@ -258,38 +285,50 @@ int tk_grad_table_destroy(tk_grad_table* table) {
   return TK_OK;
 }
 
+int tk_grad_workspace(const tk_grad_table* table, uint64_t* bytes, uint64_t* bytes_each) {
+  clear_error();
+  if (table == nullptr || bytes == nullptr || bytes_each == nullptr)
+    return set_error(TK_ERR_INVALID, "null argument");
+  *bytes_each = sizeof(double) * (tk::tiles_of(*table) + 1);
+  *bytes = tk::small(*table) ? 0 : *bytes_each;
+  return TK_OK;
+}
+
 int tk_grad_norm(const tk_grad_table* table, int32_t norm, float max_norm, float* norm_dev,
-                 float* each_dev, float* scale_dev, void* stream) {
+                 float* each_dev, float* scale_dev, void* workspace, void* stream) {
   return guarded([&] {
     TK_TRY(check_call(table, norm, false));
+    TK_TRY(check_outputs(table, {norm_dev, each_dev, scale_dev}, workspace));
     return grad_norm(*table, norm, {max_norm, norm_dev, scale_dev, nullptr}, each_dev,
-                     static_cast<cudaStream_t>(stream));
+                     workspace, static_cast<cudaStream_t>(stream));
   });
 }
 
 int tk_clip_grad_norm(const tk_grad_table* table, int32_t norm, float max_norm, float* norm_dev,
-                      float* scale_dev, void* stream) {
+                      float* scale_dev, void* workspace, void* stream) {
   return guarded([&] {
     TK_TRY(check_call(table, norm, false));
+    TK_TRY(check_outputs(table, {norm_dev, scale_dev}, workspace));
     if (!(max_norm > 0.0f))
       return set_error(TK_ERR_INVALID, "max_norm %g is not positive", (double)max_norm);
     if (!table->can_clip)
       return set_error(TK_ERR_INVALID, "a gradient that is clipped in place shares memory with "
                        "another buffer of the table");
-    return clip_grad_norm(*table, norm, {max_norm, norm_dev, scale_dev, nullptr},
+    return clip_grad_norm(*table, norm, {max_norm, norm_dev, scale_dev, nullptr}, workspace,
                           static_cast<cudaStream_t>(stream));
   });
 }
 
 int tk_accumulate_grads(const tk_grad_table* table, float alpha, int32_t overwrite, int32_t norm,
-                        float* norm_dev, void* stream) {
+                        float* norm_dev, void* workspace, void* stream) {
   return guarded([&] {
     TK_TRY(check_call(table, norm, true));
+    TK_TRY(check_outputs(table, {norm_dev}, workspace));
     if (norm != TK_NORM_NONE && norm_dev == nullptr)
       return set_error(TK_ERR_INVALID, "norm_dev is NULL");
     if (!table->can_sum)
       return set_error(TK_ERR_INVALID, "gradients are summed into f32 out buffers of their own");
-    return accumulate(*table, alpha, overwrite != 0, norm, norm_dev,
+    return accumulate(*table, alpha, overwrite != 0, norm, norm_dev, workspace,
                       static_cast<cudaStream_t>(stream));
   });
 }

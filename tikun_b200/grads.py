@@ -168,6 +168,9 @@ class GradTable:
         _on_device(self, lambda _: _native.check(
             _native.lib().tk_grad_table_create(entries, n, ctypes.byref(handle))))
         self._handle = handle
+        sizes = _native._U64(), _native._U64()
+        _native.check(_native.lib().tk_grad_workspace(handle, *map(ctypes.byref, sizes)))
+        self._scratch, self._scratch_each = (s.value for s in sizes)
         self._destroy = _native.lib().tk_grad_table_destroy
 
     def __len__(self) -> int:
@@ -184,6 +187,14 @@ class GradTable:
             self._like = torch.empty((), dtype=torch.float32, device=self.device)
             return self._like
         return torch.empty_like(self._like)  # a microsecond less
+
+    def _workspace(self, size: int):
+        """(tensor, address) of a call's scratch from torch's allocator, which
+        gives it to no other stream's work and to each captured graph its own."""
+        if not size:
+            return None, None
+        ws = torch.empty(size // 8, dtype=torch.float64, device=self.device)
+        return ws, ws.data_ptr()
 
     def _standing(self) -> "GradTable":
         for p, g in self._params:
@@ -221,8 +232,9 @@ def grad_norm(grads, norm_type: float = 2.0, per_tensor: bool = False,
     norm = t._result()
     each = torch.empty(len(t), dtype=torch.float32, device=t.device) if per_tensor else None
     each_ptr = each.data_ptr() if per_tensor and len(t) else None
+    _ws, ws = t._workspace(t._scratch_each if per_tensor else t._scratch)
     _on_device(t, lambda stream: _native.check(_native.lib().tk_grad_norm(
-        t._handle, code, 0.0, norm.data_ptr(), each_ptr, None, stream)))
+        t._handle, code, 0.0, norm.data_ptr(), each_ptr, None, ws, stream)))
     if error_if_nonfinite:
         _finite(norm, norm_type)
     return (norm, each) if per_tensor else norm
@@ -239,8 +251,9 @@ def clip_scale(grads, max_norm: float, norm_type: float = 2.0):
     t = _table(grads)
     norm = t._result()
     scale = t._result()
+    _ws, ws = t._workspace(t._scratch)
     _on_device(t, lambda stream: _native.check(_native.lib().tk_grad_norm(
-        t._handle, code, max_norm, norm.data_ptr(), None, scale.data_ptr(), stream)))
+        t._handle, code, max_norm, norm.data_ptr(), None, scale.data_ptr(), ws, stream)))
     return norm, scale
 
 
@@ -264,8 +277,9 @@ def clip_grad_norm_(grads, max_norm: float, norm_type: float = 2.0, out=None,
     if error_if_nonfinite:
         grad_norm(t, norm_type, error_if_nonfinite=True)
     norm = t._result()
+    _ws, ws = t._workspace(t._scratch)
     _on_device(t, lambda stream: _native.check(_native.lib().tk_clip_grad_norm(
-        t._handle, code, max_norm, norm.data_ptr(), None, stream)))
+        t._handle, code, max_norm, norm.data_ptr(), None, ws, stream)))
     return norm
 
 
@@ -285,8 +299,9 @@ def accumulate_grads_(grads, acc=None, alpha: float = 1.0, overwrite: bool = Fal
     t = _table(grads, acc)
     norm = t._result() if norm_type is not None else None
     norm_ptr = norm.data_ptr() if norm is not None else None
+    _ws, ws = t._workspace(t._scratch if norm is not None else 0)
     _on_device(t, lambda stream: _native.check(_native.lib().tk_accumulate_grads(
-        t._handle, alpha, 1 if overwrite else 0, code, norm_ptr, stream)))
+        t._handle, alpha, 1 if overwrite else 0, code, norm_ptr, ws, stream)))
     return norm
 
 
