@@ -315,7 +315,8 @@ struct Tile {
 // come before the one that has it.
 template <int CAP>
 __device__ __forceinline__ const GradDesc& tensor_of(const GradLaunch<CAP>& t, uint32_t at) {
-  int lo = 0, hi = t.n - 1;
+  const uint32_t k = at >> t.shift;
+  int lo = t.first[k], hi = t.first[k + 1];
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
     if (t.d[mid].t_begin <= at) lo = mid; else hi = mid - 1;
@@ -691,6 +692,13 @@ int GradPart::build(int dt, const GradDesc* d, int count, uint32_t all) {
     l->tiles = f->tiles = tiles;
     l->n = f->n = n;
     l->all_in_place = 1;
+    constexpr uint32_t kBuckets = GradLaunch<CAP>::kBuckets;
+    while (tiles > 0 && (tiles - 1) >> l->shift >= kBuckets) ++l->shift;
+    for (uint32_t k = 0, i = 0; k <= kBuckets; ++k) {
+      const uint64_t at = (uint64_t)k << l->shift;
+      while (i + 1 < (uint32_t)n && d[i + 1].t_begin <= at) ++i;
+      l->first[k] = (uint16_t)i;
+    }
     for (int i = 0; i < n; ++i) {
       l->d[i] = d[i];
       if (d[i].n && !d[i].in_place) l->all_in_place = 0;

@@ -40,13 +40,20 @@ static_assert(sizeof(GradDesc) == 32, "one descriptor is 32 bytes of kernel para
 // parameters, as the leaf tables of the step do: the smallest of three tables
 // that holds them, since a launch copies its parameters (host time of a launch
 // with 2, 10 and 31 kB of them: 3, 4 and 6 us).
+//
+// A CTA finds its tile's tensor from `first`: the tensor of every 2^shift-th
+// tile, so that one more load or two decide.  (A binary search over all of
+// them takes nine loads one after the other, each of which misses the constant
+// cache when a launch begins.)
 constexpr int kMaxGrads = 960;
 template <int CAP>
 struct GradLaunch {
+  static constexpr int kBuckets = CAP <= 64 ? 64 : 256;
   uint32_t tiles;  // of all tensors
   int32_t n;
   int32_t all_in_place;
-  int32_t reserved;
+  int32_t shift;
+  uint16_t first[kBuckets + 4];
   GradDesc d[CAP];
 };
 // What folding the tensors' own norms needs of them.
