@@ -264,6 +264,8 @@ def test_dense_views_in_other_orders():
     assert same_bits(out, clip_bits(g, norm, 1.0, torch.bfloat16))
     with pytest.raises(ValueError, match="strides"):
         clip_grad_norm_([g], 1.0, out=[torch.empty(70, 40, device="cuda")])
+    with pytest.raises(ValueError, match="lazily negated"):
+        grad_norm([torch._neg_view(w)])
     for bad in (w[:, ::2], w[:, 1:], torch.zeros(3, 1, device="cuda").expand(3, 4)):
         with pytest.raises(ValueError, match="one stretch of memory"):
             grad_norm([bad])

@@ -45,6 +45,12 @@ def _norm_code(norm_type) -> int:
     return code
 
 
+def _positive(max_norm) -> float:
+    if not max_norm > 0:
+        raise ValueError(f"max_norm is positive, got {max_norm!r}")
+    return float(max_norm)
+
+
 def _dense(t: torch.Tensor) -> bool:
     """Whether t's elements fill one stretch of memory, in whatever order."""
     if t.is_contiguous():
@@ -65,6 +71,8 @@ def _refuse(t, what: str) -> None:
         raise ValueError(f"{what}: expected a dense CUDA tensor, got {t.layout} on {t.device}")
     if t.dtype not in _DTYPES:
         raise TypeError(f"{what} is float32, bfloat16 or float16, got {t.dtype}")
+    if t.is_neg():
+        raise ValueError(f"{what} is a lazily negated view: its memory holds the negative")
     if t.numel() and not _dense(t):
         raise ValueError(f"{what}: its elements do not fill one stretch of memory (shape "
                          f"{tuple(t.shape)}, strides {t.stride()})")
@@ -76,7 +84,7 @@ def _columns(ts: list, what: str) -> tuple[list, list, list, set]:
     of the time of one tensor at a time."""
     try:
         plain = all([t.is_contiguous() for t in ts]) and all([t.is_cuda for t in ts]) and \
-            all([t.layout is torch.strided for t in ts])
+            all([t.layout is torch.strided for t in ts]) and not any([t.is_neg() for t in ts])
         codes = [_DTYPES[t.dtype] for t in ts]
     except (AttributeError, KeyError, RuntimeError):
         plain, codes = False, None
@@ -246,8 +254,7 @@ def clip_scale(grads, max_norm: float, norm_type: float = 2.0):
     The optimizers' ``step(clip_scale=scale)`` folds it into their updates, so
     that several of them clip by one norm and no gradient is written."""
     code = _norm_code(norm_type)
-    if not max_norm > 0:
-        raise ValueError(f"max_norm is positive, got {max_norm!r}")
+    max_norm = _positive(max_norm)
     t = _table(grads)
     norm = t._result()
     scale = t._result()
@@ -271,8 +278,7 @@ def clip_grad_norm_(grads, max_norm: float, norm_type: float = 2.0, out=None,
     ``error_if_nonfinite=True`` raises ``RuntimeError`` for both before
     anything is written, and waits for the norm to know."""
     code = _norm_code(norm_type)
-    if not max_norm > 0:
-        raise ValueError(f"max_norm is positive, got {max_norm!r}")
+    max_norm = _positive(max_norm)
     t = _table(grads, out)
     if error_if_nonfinite:
         grad_norm(t, norm_type, error_if_nonfinite=True)
@@ -301,7 +307,7 @@ def accumulate_grads_(grads, acc=None, alpha: float = 1.0, overwrite: bool = Fal
     norm_ptr = norm.data_ptr() if norm is not None else None
     _ws, ws = t._workspace(t._scratch if norm is not None else 0)
     _on_device(t, lambda stream: _native.check(_native.lib().tk_accumulate_grads(
-        t._handle, alpha, 1 if overwrite else 0, code, norm_ptr, ws, stream)))
+        t._handle, float(alpha), 1 if overwrite else 0, code, norm_ptr, ws, stream)))
     return norm
 
 
