@@ -190,6 +190,10 @@ def test_types_mixed_in_one_call():
     assert same_bits(norm, got)
     for t, o in zip(ts, outs):
         assert same_bits(o, clip_bits(t, norm, 1.0, o.dtype))
+    before = [t.clone() for t in ts]
+    assert same_bits(clip_grad_norm_(ts, 1.0), norm)
+    for t, b in zip(ts, before):
+        assert same_bits(t, clip_bits(b, norm, 1.0, t.dtype))
 
 
 @pytest.mark.parametrize("p", NORMS)
@@ -559,6 +563,29 @@ def test_captured_calls_and_graphs_side_by_side():
             for t, o, x in zip(ts, outs, each.tolist()):
                 assert same_bits(o, clip_bits(t, norm, 0.01, torch.float32))
                 assert_norm(x, norm64([t], 2.0), torch.bfloat16, 2.0)
+
+
+@pytest.mark.parametrize("limit", [0.5, 2.0], ids=["over", "under"])
+def test_captured_clip_in_place_replays(limit):
+    """Every replay of a clip in place scales each element once."""
+    sizes = [700_001, 768, 0, 1_300_000]
+    ts = [t for d in DTYPES for t in tensors(sizes, d, offsets=(0, 3))]
+    table = GradTable(ts)
+    clip_grad_norm_(table, 1.0)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        norm = clip_grad_norm_(table, limit)
+    for round_ in range(3):
+        fresh = [t for d in DTYPES for t in tensors(sizes, d, seed=round_, std=1.0 / 2400)]
+        for t, f in zip(ts, fresh):
+            t.copy_(f)
+        g.replay()
+        torch.cuda.synchronize()
+        assert_norm(norm, norm64(fresh, 2.0), torch.bfloat16, 2.0)
+        assert (norm.item() > limit) == (limit == 0.5)
+        for t, f in zip(ts, fresh):
+            assert same_bits(t, clip_bits(f, norm, limit, t.dtype))
 
 
 def test_streams_and_threads():

@@ -51,8 +51,8 @@ struct GradLaunch {
   static constexpr int kBuckets = CAP <= 64 ? 64 : 256;
   uint32_t tiles;  // of all tensors
   int32_t n;
-  int32_t all_in_place;
   int32_t shift;
+  int32_t reserved;
   uint16_t first[kBuckets + 4];
   GradDesc d[CAP];
 };
@@ -71,6 +71,7 @@ struct GradPart {  // host side: one launch
   int n = 0;
   uint32_t tiles = 0;
   uint64_t units = 0;
+  bool all_in_place = true;             // so is what clipping writes
   int cap = 0;                          // 64, 320 or kMaxGrads
   std::unique_ptr<uint64_t[]> launch;   // GradLaunch<cap>
   std::unique_ptr<uint64_t[]> fold;     // FoldLaunch<cap>
@@ -95,7 +96,10 @@ struct NormOut {
   float max_norm = 0.0f;
   float* norm = nullptr;
   float* scale = nullptr;
+  // for launch_clip: the scale again, and a counter per part, set to 0
   float* scale_too = nullptr;
+  uint32_t* tickets = nullptr;
+  int n_tickets = 0;
 };
 // Both from n partials.  Enqueued right behind the launches that write them.
 int launch_fold(int norm, const double* partials, int64_t n, const NormOut& out, cudaStream_t s);
@@ -103,8 +107,9 @@ int launch_fold(int norm, const double* partials, int64_t n, const NormOut& out,
 // the norm of n partials from `all` too.
 int launch_fold_each(const GradPart& p, int norm, const double* partials, float* each,
                      const double* all, int64_t n, const NormOut* out, cudaStream_t s);
-// out = *scale g.  Enqueued right behind the launch that writes *scale.
-int launch_clip(const GradPart& p, const float* scale, cudaStream_t s);
+// out = *scale g.  Enqueued right behind the launch that writes *scale and sets
+// *ticket to 0.
+int launch_clip(const GradPart& p, const float* scale, uint32_t* ticket, cudaStream_t s);
 
 // A whole call in one launch, for a table of one part and few tiles (small).
 bool small(const GradPart& p);

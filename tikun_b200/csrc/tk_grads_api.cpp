@@ -160,6 +160,10 @@ size_t tiles_of(const tk_grad_table& t) {
   return n;
 }
 
+// f64 words that a clip needs: the partials, and behind them the scale and a
+// ticket per part, four bytes each.  No call needs more.
+size_t clip_words(const tk_grad_table& t) { return tiles_of(t) + (t.parts.size() + 2) / 2; }
+
 // Every part's partials, one after the other.
 int norm_parts(const tk_grad_table& t, int norm, bool again, double* partials, cudaStream_t s) {
   for (const auto& p : t.parts) {
@@ -209,12 +213,14 @@ int clip_grad_norm(const tk_grad_table& t, int norm, gr::NormOut out, void* work
   const size_t total = tiles_of(t);
   Scratch pool;
   double* partials = nullptr;
-  TK_TRY(scratch(workspace, total + 1, &pool, s, &partials));
+  TK_TRY(scratch(workspace, clip_words(t), &pool, s, &partials));
   out.scale_too = reinterpret_cast<float*>(partials + total);
+  out.tickets = reinterpret_cast<uint32_t*>(out.scale_too + 1);
+  out.n_tickets = (int)t.parts.size();
   TK_TRY(norm_parts(t, norm, true, partials, s));
   TK_TRY(gr::launch_fold(norm, partials, (int64_t)total, out, s));
   for (size_t i = t.parts.size(); i-- > 0;)  // the norm's last part first
-    if (t.parts[i].tiles) TK_TRY(gr::launch_clip(t.parts[i], out.scale_too, s));
+    if (t.parts[i].tiles) TK_TRY(gr::launch_clip(t.parts[i], out.scale_too, out.tickets + i, s));
   return TK_OK;
 }
 
@@ -289,7 +295,7 @@ int tk_grad_workspace(const tk_grad_table* table, uint64_t* bytes, uint64_t* byt
   clear_error();
   if (table == nullptr || bytes == nullptr || bytes_each == nullptr)
     return set_error(TK_ERR_INVALID, "null argument");
-  *bytes_each = sizeof(double) * (tk::tiles_of(*table) + 1);
+  *bytes_each = sizeof(double) * tk::clip_words(*table);
   *bytes = tk::small(*table) ? 0 : *bytes_each;
   return TK_OK;
 }
