@@ -380,6 +380,23 @@ def test_parameters_stand_for_their_gradients():
     assert grad_norm(lin.parameters()).item() == 0.0
 
 
+def test_a_table_keeps_its_memory_and_is_not_copied():
+    import copy
+    import pickle
+
+    g = torch.full((1 << 20,), 2.0, device="cuda")
+    table = GradTable([g])
+    g.data = torch.zeros(4, device="cuda")
+    junk = [torch.full((1 << 20,), 9.0, device="cuda") for _ in range(4)]
+    assert grad_norm(table, norm_type=1.0).item() == 2.0 * (1 << 20) and len(junk) == 4
+    for dup in (copy.copy, copy.deepcopy, pickle.dumps):
+        with pytest.raises(TypeError, match="build another"):
+            dup(table)
+    p = torch.nn.Parameter(torch.zeros(1 << 20, device="cuda"))
+    with pytest.raises(TypeError, match="not parameters"):
+        GradTable(table.grads, out=[p])
+
+
 def test_micro_batches_norm_clip_and_step_together():
     """Sum, norm, clip and an AdamW step that does not clip give the bits of the
     fused clipped step on the same sums; the clipped bf16 gradients, too, of

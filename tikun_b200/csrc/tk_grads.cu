@@ -279,7 +279,8 @@ __device__ __forceinline__ double cluster_join(double x) {
 }
 
 constexpr int kFoldThreads = 512;
-// partials[i] for i = first, first + step, ..: valid in thread 0.
+// The join of n partials in one CTA, or this CTA's part of it; valid in
+// thread 0.
 template <int NORM>
 __device__ __forceinline__ double fold(const double* __restrict__ partials, int64_t n,
                                        int part = 0, int parts = 1) {

@@ -12,7 +12,6 @@
 
 struct tk_grad_table {
   int dev = 0;
-  size_t n = 0;
   bool can_clip = false;  // no buffer that clipping writes shares memory with another
   bool can_sum = false;   // every out is f32 and not its own g
   std::vector<tk::gr::GradPart> parts;  // one launch each
@@ -63,7 +62,6 @@ int create(const tk_grad* grads, size_t n, tk_grad_table** out) {
   *out = nullptr;
   if (n > 0 && grads == nullptr) return set_error(TK_ERR_INVALID, "grads is NULL with n=%zu", n);
   auto t = std::make_unique<tk_grad_table>();
-  t->n = n;
   t->can_sum = true;
   // A gradient in place counts as read only in `ranges`, as written in
   // `clipped`: a norm may be taken of one tensor given twice, but clipping it
