@@ -270,6 +270,11 @@ def test_dense_views_in_other_orders():
         clip_grad_norm_([g], 1.0, out=[torch.empty(70, 40, device="cuda")])
     with pytest.raises(ValueError, match="lazily negated"):
         grad_norm([torch._neg_view(w)])
+    for sparse in (w.to_sparse(), w.to_sparse_csr()):
+        with pytest.raises(ValueError, match="dense CUDA tensor"):
+            grad_norm([w, sparse])
+    with pytest.raises(ValueError, match="dense CUDA tensor"):
+        grad_norm([w, torch.empty(3, device="meta")])
     for bad in (w[:, ::2], w[:, 1:], torch.zeros(3, 1, device="cuda").expand(3, 4)):
         with pytest.raises(ValueError, match="one stretch of memory"):
             grad_norm([bad])

@@ -80,20 +80,22 @@ def _refuse(t, what: str) -> None:
 
 def _columns(ts: list, what: str) -> tuple[list, list, list, set, bool]:
     """Addresses, element counts and type codes of checked tensors, their
-    device indices, and whether all are contiguous.  One attribute of all tensors at a time, which takes a third
-    of the time of one tensor at a time."""
+    device indices, and whether all are contiguous.  One attribute of all
+    tensors at a time: a third of the time of one tensor at a time."""
+    at = None
     try:
-        plain = all([t.is_contiguous() for t in ts]) and all([t.is_cuda for t in ts]) and \
-            all([t.layout is torch.strided for t in ts]) and not any([t.is_neg() for t in ts])
-        codes = [_DTYPES[t.dtype] for t in ts]
-    except (AttributeError, KeyError, RuntimeError):
-        plain, codes = False, None
+        at, codes = [t.data_ptr() for t in ts], [_DTYPES[t.dtype] for t in ts]
+        devices = {t.get_device() for t in ts}  # -1 on the host
+        plain = min(devices, default=0) >= 0 and all([t.is_contiguous() for t in ts]) and \
+            not any([t.is_neg() for t in ts])
+    except (AttributeError, KeyError, RuntimeError):  # no tensor, its type, no memory of its own
+        plain = False
     if not plain:
         for i, t in enumerate(ts):
             _refuse(t, f"{what} {i}")
-        codes = [_DTYPES[t.dtype] for t in ts]
-    return ([t.data_ptr() for t in ts], [t.numel() for t in ts], codes,
-            {t.get_device() for t in ts}, plain)
+        if at is None:
+            raise TypeError(f"the {what} tensors have no memory of their own")
+    return at, [t.numel() for t in ts], codes, devices, plain
 
 
 # what current_stream().cuda_stream gives, at a fortieth of its 3 us
