@@ -5,9 +5,9 @@ of f32):
 
 * norm: f32 elements are squared exactly and summed in f64, so that only the
   last rounding to f32 is left: u.  bf16 and f16 elements are first added by
-  eights in f32, at most five roundings for a group's sum, which is 5 u of an L1
-  norm and half of that of an L2 norm: 6 u with the last one.  The largest
-  magnitude is exact.
+  eights in f32 as two chains of four and their sum, at most four roundings on
+  the way of each value, which is 4 u of an L1 norm and half of that of an L2
+  norm: 5 u with the last one.  The largest magnitude is exact.
 * clipping: given the norm, scale and products are separately rounded f32
   operations: equal bits.
 * the sum over micro-batches: one f32 rounding of alpha * g + acc: u, and half
@@ -63,7 +63,7 @@ def assert_norm(got, want, dtype, p):
     if math.isnan(want) or math.isinf(want) or p == math.inf:
         assert got == want or (math.isnan(got) and math.isnan(want)), (got, want)
         return
-    tol = (1 if dtype == torch.float32 else 6) * U * 1.001
+    tol = (1 if dtype == torch.float32 else 5) * U * 1.001
     assert abs(got - want) <= tol * want + 2.0 ** -150, (got, want, abs(got - want) / max(want, 1e-300))
 
 
