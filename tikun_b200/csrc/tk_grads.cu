@@ -49,13 +49,19 @@ constexpr int kThreads = 256;
 constexpr int kMaxCluster = 8;  // the largest that every device setting allows
 
 // Calls of at most so many tiles and units are one launch of one cluster
-// (small_kernel).  Measured on tables of 768-element tensors, a clip, time per
-// call without torch (the host's and the device's overlap): 64 tensors 8.2 us
-// against 10.2 us in three launches, 128 tensors 12.3 against 9.0; on whole
-// tiles, 32 of them 8.2 against 8.8 us, 64 of them 12.6 against 8.8.
-constexpr uint32_t kSmallTiles = 64;
+// (small_kernel).  A clip through the Python functions, us a call among others,
+// so against in two launches: 32 whole f32 tiles 8.2 and 11.4, 48 of them 12.2
+// and 11.1; 96 tensors of 768 elements 8.2 and 11.7, 128 of them 10.3 and 11.7
+// (alone, with the wait for it, 20.4 and 19.9, 21.4 and 19.3).
+constexpr uint32_t kSmallTiles = 96;
 constexpr uint64_t kSmallUnits = 32 * 1024;
 constexpr int kSmallThreads = 1024;
+
+// Up to so many tiles every CTA of a clip's scaling folds the norm's partials
+// for itself, which saves a launch.  C calls, us, so against with a fold
+// between: 96 whole f32 tiles 7.0 and 9.5, 592 of them 14.4 and 16.2, 1200 of
+// them 21.4 and 22.7, 2441 of them 42.1 and 41.0.
+constexpr uint32_t kSelfFoldTiles = 1200;
 
 // ------------------------------------------------------------------ dependent launches
 __device__ __forceinline__ void let_next_start() {
@@ -587,6 +593,38 @@ clip_kernel(const __grid_constant__ GradLaunch<CAP> t, const float* __restrict__
   });
 }
 
+// The same behind the norm itself, for few partials; CTA 0 reports them.
+template <int CAP, int GDT>
+__global__ void __launch_bounds__(kThreads, 5)
+fold_clip_kernel(const __grid_constant__ GradLaunch<CAP> t, int norm,
+                 const double* __restrict__ partials, const NormOut out) {
+  __shared__ float s_scale;
+  const uint32_t at = t.tiles - 1 - blockIdx.x;
+  const GradDesc& d = tensor_of(t, at);
+  wait_for_previous();
+  auto scale_of = [&](auto k) {
+    constexpr int NORM = decltype(k)::value;
+    double v = 0.0;
+#pragma unroll 4
+    for (uint32_t i = threadIdx.x; i < t.tiles; i += kThreads) v = join<NORM>(v, partials[i]);
+    v = block_join<NORM, kThreads>(v);
+    if (threadIdx.x == 0) {
+      const float n = root<NORM>(v);
+      s_scale = clip_scale(n, out.max_norm);
+      if (blockIdx.x == 0) report(out, n, s_scale);
+    }
+  };
+  if (norm == TK_NORM_L2) scale_of(Const<TK_NORM_L2>{});
+  else if (norm == TK_NORM_L1) scale_of(Const<TK_NORM_L1>{});
+  else scale_of(Const<TK_NORM_MAX>{});
+  __syncthreads();
+  const float scale = s_scale;
+  if (scale == 1.0f && d.in_place) return;
+  with_dtype(d.out_dtype, [&](auto odt) {
+    clip_tile<GDT, decltype(odt)::value, 4>(d, at, scale);
+  });
+}
+
 // The same where every tensor is in place, so that a scale of 1, which most
 // steps of a run have, leaves nothing to do at all: one resident wave of CTAs
 // that take tile after tile by a ticket, since 15,000 CTAs that only find that
@@ -802,6 +840,21 @@ int launch_clip(const GradPart& p, const float* scale, uint32_t* ticket, cudaStr
       void* args[] = {p.launch.get(), at(scale)};
       return gr::launch((const void*)clip_kernel<decltype(c)::value, decltype(dt)::value>, p.tiles,
                         kThreads, 1, true, args, s);
+    });
+  });
+}
+
+bool folds_itself(const GradPart& p) {
+  return p.tiles <= kSelfFoldTiles;
+}
+
+int launch_fold_clip(const GradPart& p, int norm, const double* partials, const NormOut& out,
+                     cudaStream_t s) {
+  return with_cap(p.cap, [&](auto c) {
+    return with_g_dtype(p.g_dtype, [&](auto dt) {
+      void* args[] = {p.launch.get(), at(norm), at(partials), at(out)};
+      return gr::launch((const void*)fold_clip_kernel<decltype(c)::value, decltype(dt)::value>,
+                        p.tiles, kThreads, 1, true, args, s);
     });
   });
 }

@@ -107,6 +107,12 @@ int launch_fold(int norm, const double* partials, int64_t n, const NormOut& out,
 // the norm of n partials from `all` too.
 int launch_fold_each(const GradPart& p, int norm, const double* partials, float* each,
                      const double* all, int64_t n, const NormOut* out, cudaStream_t s);
+// Whether so few partials are folded by every CTA of the scaling itself, in
+// place of launch_fold.
+bool folds_itself(const GradPart& p);
+// out = scale g, with the scale of the partials that the launch before wrote.
+int launch_fold_clip(const GradPart& p, int norm, const double* partials, const NormOut& out,
+                     cudaStream_t s);
 // out = *scale g.  Enqueued right behind the launch that writes *scale and sets
 // *ticket to 0.
 int launch_clip(const GradPart& p, const float* scale, uint32_t* ticket, cudaStream_t s);

@@ -212,6 +212,10 @@ int clip_grad_norm(const tk_grad_table& t, int norm, gr::NormOut out, void* work
   Scratch pool;
   double* partials = nullptr;
   TK_TRY(scratch(workspace, clip_words(t), &pool, s, &partials));
+  if (t.parts.size() == 1 && gr::folds_itself(t.parts[0])) {
+    TK_TRY(norm_parts(t, norm, true, partials, s));
+    return gr::launch_fold_clip(t.parts[0], norm, partials, out, s);
+  }
   out.scale_too = reinterpret_cast<float*>(partials + total);
   out.tickets = reinterpret_cast<uint32_t*>(out.scale_too + 1);
   out.n_tickets = (int)t.parts.size();
