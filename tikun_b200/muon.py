@@ -67,7 +67,8 @@ class Muon(torch.optim.Optimizer):
             check_clip_scale(clip_scale, self.max_norm)
         elif self.max_norm > 0:
             params = self.param_groups[0]["params"] + (self.adamw.params if self.adamw else [])
-            self.grad_norm, clip_scale = scale_of([p.grad for p in params], self.max_norm)
+            self.grad_norm, clip_scale = scale_of([getattr(p, "grad", None) for p in params],
+                                                  self.max_norm)
         self.clip_scale = clip_scale
         self.step_count += 1
         leaves = []
