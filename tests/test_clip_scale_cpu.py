@@ -1,0 +1,108 @@
+"""What the optimizers do with a clip scale of the caller's, seen from the host:
+stand-ins for CUDA tensors, and the native calls recorded in place of run."""
+import contextlib
+
+import pytest
+import torch
+
+import tikun_b200
+from tikun_b200 import _native
+from tikun_b200.optimizer import AdamW as TorchAdamW
+
+
+class OnDevice(torch.Tensor):
+    """A host tensor that says it is a CUDA tensor; `dev` stands for its device."""
+    is_cuda = property(lambda self: True)
+    device = property(lambda self: getattr(self, "dev", torch.device("cpu")))
+
+
+def on_device(data, dev=None):
+    t = torch.as_tensor(data, dtype=torch.float32).clone().as_subclass(OnDevice)
+    if dev is not None:
+        t.dev = torch.device(dev)
+    return t
+
+
+def leaf(*shape, dev=None):
+    p = on_device(torch.randn(*shape)).requires_grad_()
+    p.grad = torch.ones(*shape).as_subclass(OnDevice)
+    if dev is not None:
+        p.dev = torch.device(dev)
+    return p
+
+
+class Calls(list):
+    """(entry point, address that it reads or writes its scale at) of each call."""
+
+    def record(self, name):
+        def call(*args, **kw):
+            at = kw["clip_scale_ptr"] if "clip_scale_ptr" in kw else args[-1]
+            self.append((name, at))
+
+        return call
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    got = Calls()
+    for name in ("apply_pointwise", "step_fast_buffers_async", "muon_step"):
+        monkeypatch.setattr(_native, name, got.record(name))
+    monkeypatch.setattr(torch.cuda, "device", lambda dev: contextlib.nullcontext())
+    return got
+
+
+FORMS = {
+    "universal": lambda ps: tikun_b200.AdamW(ps),
+    "lion": lambda ps: tikun_b200.Lion(ps),
+    "torch": lambda ps: TorchAdamW(ps),
+}
+
+
+def set_max_norm(opt, value):
+    if isinstance(opt, TorchAdamW):
+        opt.param_groups[0]["max_norm"] = value
+    else:
+        opt.max_norm = value
+
+
+@pytest.mark.parametrize("max_norm", [0.0, 1.0])
+@pytest.mark.parametrize("form", FORMS)
+def test_a_step_without_a_scale_writes_none_of_the_callers(calls, form, max_norm):
+    opt = FORMS[form]([leaf(5), leaf(2, 3)])
+    scale = on_device(0.25)
+    opt.step(clip_scale=scale)
+    assert calls == [("apply_pointwise", scale.data_ptr())] and opt.clip_scale is scale
+    set_max_norm(opt, max_norm)
+    opt.step()
+    name, at = calls[-1]
+    assert name == "step_fast_buffers_async" and at != scale.data_ptr()
+    assert opt.clip_scale is not scale and opt.clip_scale.data_ptr() == at
+    own = opt.clip_scale
+    opt.step()
+    assert calls[-1][1] == own.data_ptr() and opt.clip_scale is own
+
+
+@pytest.mark.parametrize("form", ["muon", "muon_nd"])
+def test_muon_hands_its_adamw_no_buffer_of_the_callers(calls, form):
+    w, b = leaf(4, 6), leaf(6)
+    opt = tikun_b200.Muon([w], [b]) if form == "muon" else tikun_b200.MuonND([w, b])
+    scale = on_device(0.25)
+    opt.step(clip_scale=scale)
+    assert sorted(calls) == [("apply_pointwise", scale.data_ptr()), ("muon_step", scale.data_ptr())]
+    assert opt.clip_scale is scale
+    calls.clear()
+    opt.step()
+    assert opt.clip_scale is None
+    got = dict(calls)
+    assert got["muon_step"] == 0 and got["step_fast_buffers_async"] != scale.data_ptr()
+
+
+def test_host_and_device_leaves_in_one_in_backward_optimizer(calls, monkeypatch):
+    """The scale of a host leaf is a number, which no device step takes for its buffer."""
+    monkeypatch.setattr(_native, "step_fast_buffers", lambda *args, **kw: 1.0)
+    host, dev = torch.nn.Parameter(torch.ones(3)), leaf(4)
+    opt = tikun_b200.AdamW([host, dev], in_backward=True)
+    host.sum().backward()
+    assert opt.clip_scale == 1.0
+    opt._step_single_tensor(dev)
+    assert calls[-1] == ("step_fast_buffers_async", opt.clip_scale.data_ptr())

@@ -36,6 +36,7 @@ class AdamW(torch.optim.Optimizer):
         super().__init__(params, defaults)
         self.step_count = 0
         self.clip_scale = None
+        self._own_scale = None  # where the engine writes it; never a tensor of the caller's
 
     def state_dict(self) -> dict:
         """torch's state (m1 and m2 per parameter) plus the step counter."""
@@ -107,12 +108,12 @@ class AdamW(torch.optim.Optimizer):
             self.clip_scale = clip_scale
         elif len(devices) == 1 and params[0].is_cuda:
             dev = params[0].device
-            if self.clip_scale is None or not isinstance(self.clip_scale, torch.Tensor) or \
-                    self.clip_scale.device != dev:
-                self.clip_scale = torch.ones((), dtype=torch.float32, device=dev)
+            if self._own_scale is None or self._own_scale.device != dev:
+                self._own_scale = torch.ones((), dtype=torch.float32, device=dev)
             with torch.cuda.device(dev):
-                _native.step_fast_buffers_async(*args, clip_scale_ptr=self.clip_scale.data_ptr(),
+                _native.step_fast_buffers_async(*args, clip_scale_ptr=self._own_scale.data_ptr(),
                                                 p_dtypes=p_dt, g_dtypes=g_dt)
+            self.clip_scale = self._own_scale
         else:
             self.clip_scale = _native.step_fast_buffers(*args, p_dtypes=p_dt, g_dtypes=g_dt,
                                                         stream=0)

@@ -139,7 +139,9 @@ class UniversalOptimizer:
         self.in_backward = in_backward
         self.m1_state: dict[int, Any] = {}
         self.m2_state: dict[int, Any] = {}
-        self.clip_scale = None  # device f32 tensor (CUDA params) or float (host params)
+        # the last step's: device f32 tensor (CUDA params) or float (host params)
+        self.clip_scale = None
+        self._own_scale = None  # where the engine writes it; never a tensor of the caller's
         self._arena = None
         if arena:
             if in_backward:
@@ -187,13 +189,14 @@ class UniversalOptimizer:
         elif on_device:
             import torch
 
-            if self.clip_scale is None or self.clip_scale.device != device:
-                self.clip_scale = torch.ones((), dtype=torch.float32, device=device)
+            if self._own_scale is None or self._own_scale.device != device:
+                self._own_scale = torch.ones((), dtype=torch.float32, device=device)
             with torch.cuda.device(device):
                 _native.step_fast_buffers_async(
                     p_ptrs, g_ptrs, m1_ptrs, m2_ptrs, lengths, self.max_norm, self.algorithm,
                     step, self.lr, self.beta1, self.beta2, self.eps, self.weight_decay,
-                    clip_scale_ptr=self.clip_scale.data_ptr(), p_dtypes=p_dt, g_dtypes=g_dt)
+                    clip_scale_ptr=self._own_scale.data_ptr(), p_dtypes=p_dt, g_dtypes=g_dt)
+            self.clip_scale = self._own_scale
         else:
             self.clip_scale = _native.step_fast_buffers(
                 p_ptrs, g_ptrs, m1_ptrs, m2_ptrs, lengths, self.max_norm, self.algorithm, step,
