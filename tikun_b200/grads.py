@@ -134,7 +134,8 @@ class GradTable:
     ``accumulate_grads_`` write; without it they work in place.  The table reads
     and writes the memory that the tensors have now, and keeps it.  For
     parameters it is their ``.grad`` of now: a call raises ``RuntimeError`` once
-    one of them has another (as after ``zero_grad(set_to_none=True)``)."""
+    one of them has another (as after ``zero_grad(set_to_none=True)``), or has
+    its first."""
 
     def __init__(self, grads, out=None):
         self._build(grads, out)
@@ -153,8 +154,8 @@ class GradTable:
             for leaf in leaves:
                 if isinstance(leaf, torch.nn.Parameter):
                     g = leaf.grad
+                    self._params.append((leaf, g))  # without one too: it may get its first
                     if g is not None:
-                        self._params.append((leaf, g))
                         self.grads.append(g)
                 elif leaf is not None:
                     self.grads.append(leaf)
