@@ -96,9 +96,9 @@ struct NormOut {
   float max_norm = 0.0f;
   float* norm = nullptr;
   float* scale = nullptr;
-  // for launch_clip: the scale again, and a counter per part, set to 0
-  float* scale_too = nullptr;
-  uint32_t* tickets = nullptr;
+  // for launch_clip: the scale again, and behind it a counter per part, set to 0;
+  // aligned to 32 bytes, with room to a multiple of them
+  float* line = nullptr;
   int n_tickets = 0;
 };
 // Both from n partials.  Enqueued right behind the launches that write them.

@@ -159,8 +159,18 @@ size_t tiles_of(const tk_grad_table& t) {
 }
 
 // f64 words that a clip needs: the partials, and behind them the scale and a
-// ticket per part, four bytes each.  No call needs more.
-size_t clip_words(const tk_grad_table& t) { return tiles_of(t) + (t.parts.size() + 2) / 2; }
+// ticket per part, four bytes each, on 128-byte lines of their own: the scale is
+// written while CTAs of the same launch read the last partials, and read by CTAs
+// that are resident by then.  No call needs more.
+constexpr size_t kLineWords = 16;
+size_t clip_words(const tk_grad_table& t) {
+  const size_t lines = ((1 + t.parts.size()) * 4 + 127) / 128;
+  return tiles_of(t) + kLineWords - 1 + lines * kLineWords;
+}
+float* scale_line(double* partials, size_t total) {
+  const uintptr_t end = reinterpret_cast<uintptr_t>(partials + total);
+  return reinterpret_cast<float*>((end + 127) / 128 * 128);
+}
 
 // Every part's partials, one after the other.
 int norm_parts(const tk_grad_table& t, int norm, bool again, double* partials, cudaStream_t s) {
@@ -216,13 +226,13 @@ int clip_grad_norm(const tk_grad_table& t, int norm, gr::NormOut out, void* work
     TK_TRY(norm_parts(t, norm, true, partials, s));
     return gr::launch_fold_clip(t.parts[0], norm, partials, out, s);
   }
-  out.scale_too = reinterpret_cast<float*>(partials + total);
-  out.tickets = reinterpret_cast<uint32_t*>(out.scale_too + 1);
+  out.line = scale_line(partials, total);
+  uint32_t* tickets = reinterpret_cast<uint32_t*>(out.line + 1);
   out.n_tickets = (int)t.parts.size();
   TK_TRY(norm_parts(t, norm, true, partials, s));
   TK_TRY(gr::launch_fold(norm, partials, (int64_t)total, out, s));
   for (size_t i = t.parts.size(); i-- > 0;)  // the norm's last part first
-    if (t.parts[i].tiles) TK_TRY(gr::launch_clip(t.parts[i], out.scale_too, out.tickets + i, s));
+    if (t.parts[i].tiles) TK_TRY(gr::launch_clip(t.parts[i], out.line, tickets + i, s));
   return TK_OK;
 }
 
