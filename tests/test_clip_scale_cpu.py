@@ -2,6 +2,7 @@
 stand-ins for CUDA tensors, and the native calls recorded in place of run."""
 import contextlib
 
+import numpy as np
 import pytest
 import torch
 
@@ -106,3 +107,73 @@ def test_host_and_device_leaves_in_one_in_backward_optimizer(calls, monkeypatch)
     assert opt.clip_scale == 1.0
     opt._step_single_tensor(dev)
     assert calls[-1] == ("step_fast_buffers_async", opt.clip_scale.data_ptr())
+
+
+def state_of(opt, params):
+    inner = [o for o in (opt, getattr(opt, "adamw", None), getattr(opt, "_adamw", None)) if o]
+    return ([o.step_count for o in inner], opt.clip_scale, [p.detach().clone() for p in params])
+
+
+@pytest.mark.parametrize("odd", ["first", "last"])
+@pytest.mark.parametrize("form", [*FORMS, "muon", "muon_nd"])
+def test_a_scale_on_another_device_is_refused_before_anything_changes(calls, form, odd):
+    """Also where it is on the device of some of the leaves only."""
+    ps = [leaf(4, 6), leaf(6, 2), leaf(6), leaf(3)]
+    build = {**FORMS, "muon": lambda ps: tikun_b200.Muon(ps[:2], ps[2:]),
+             "muon_nd": lambda ps: tikun_b200.MuonND(ps)}[form]
+    opt = build(ps)
+    ps[0 if odd == "first" else -1].dev = torch.device("cuda", 1)
+    before = state_of(opt, ps)
+    for scale in (on_device(0.5), on_device(0.5, "cuda:1"), on_device(0.5, "cuda:2")):
+        with pytest.raises(ValueError, match="on the device of the parameters"):
+            opt.step(clip_scale=scale)
+    assert calls == []
+    after = state_of(opt, ps)
+    assert after[:2] == before[:2] and all(torch.equal(x, y) for x, y in zip(after[2], before[2]))
+    assert not getattr(opt, "m1_state", None) and not getattr(opt, "momentum_state", None)
+    # a leaf that is not stepped may be anywhere
+    if form != "torch":  # which refuses a missing gradient
+        ps[0 if odd == "first" else -1].grad = None
+        opt.step(clip_scale=on_device(0.5))
+        assert calls and opt.step_count == before[0][0] + 1
+
+
+def test_a_scale_is_refused_for_host_leaves(calls):
+    """Arrays and address pairs too, with the gradients given."""
+    w = np.ones(4, np.float32)
+    g = np.ones(4, np.float32)
+    opt = tikun_b200.AdamW([w, (w.ctypes.data, 4)])
+    with pytest.raises(ValueError, match="on the device of the parameters"):
+        opt.step([g, g], clip_scale=on_device(0.5))
+    p = torch.nn.Parameter(torch.ones(4))
+    p.grad = torch.ones(4)
+    for opt in (tikun_b200.SGD([p]), tikun_b200.MuonND([p]), TorchAdamW([p])):
+        with pytest.raises(ValueError, match="on the device of the parameters"):
+            opt.step(clip_scale=on_device(0.5, "cuda:0"))
+        assert opt.step_count == 0
+    assert calls == []
+
+
+def test_an_arena_takes_no_gradients_with_a_refused_scale(calls, monkeypatch):
+    from tikun_b200 import universal
+
+    copied = []
+
+    class Arena:
+        def __init__(self, params):
+            self.device = torch.device("cpu")
+
+        def moments(self):
+            return []
+
+        def step(self, opt, grads, clip_scale):
+            copied.append(grads)
+
+    monkeypatch.setattr(universal, "_ArenaState", Arena)
+    p = leaf(4)
+    opt = tikun_b200.AdamW([p], arena=True)
+    with pytest.raises(ValueError, match="on the device of the parameters"):
+        opt.step([torch.ones(4)], clip_scale=on_device(0.5, "cuda:1"))
+    assert copied == [] and opt.step_count == 0
+    opt.step([torch.ones(4)], clip_scale=on_device(0.5))
+    assert len(copied) == 1 and opt.step_count == 1

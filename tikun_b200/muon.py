@@ -18,7 +18,7 @@ import torch
 from . import _native
 from .grads import clip_scale as scale_of
 from .muon_nd import MultiDimensionalMuon
-from .universal import UniversalOptimizer, _tk_dtype, check_clip_scale
+from .universal import UniversalOptimizer, _tk_dtype, check_clip_scale, with_gradient
 
 
 def zeropower_via_newtonschulz5(G: torch.Tensor, steps: int = 5, eps: float = 1e-7,
@@ -63,12 +63,13 @@ class Muon(torch.optim.Optimizer):
     @torch.no_grad()
     def step(self, clip_scale=None):
         """muon.py:79-102.  ``clip_scale``: see ``MultiDimensionalMuon.step``."""
-        if clip_scale is not None:
-            check_clip_scale(clip_scale, self.max_norm)
-        elif self.max_norm > 0:
-            params = self.param_groups[0]["params"] + (self.adamw.params if self.adamw else [])
-            self.grad_norm, clip_scale = scale_of([getattr(p, "grad", None) for p in params],
-                                                  self.max_norm)
+        if clip_scale is not None or self.max_norm > 0:
+            params = with_gradient(self.param_groups[0]["params"] +
+                                   (self.adamw.params if self.adamw else []))
+            if clip_scale is not None:
+                check_clip_scale(clip_scale, params, self.max_norm)
+            else:
+                self.grad_norm, clip_scale = scale_of([p.grad for p in params], self.max_norm)
         self.clip_scale = clip_scale
         self.step_count += 1
         leaves = []

@@ -36,7 +36,7 @@ import numpy as np
 
 from . import _native
 from .universal import (UniversalOptimizer, _extract_pointer_and_len, _flatten_pytree, _tk_dtype,
-                        check_clip_scale)
+                        check_clip_scale, with_gradient)
 
 
 def _ndim(p) -> int:
@@ -102,12 +102,12 @@ class MultiDimensionalMuon:
         ``grads.clip_scale`` returns it): the scale of a norm over more gradients
         than this optimizer's."""
         if clip_scale is not None:
-            check_clip_scale(clip_scale, self.max_norm)
+            check_clip_scale(clip_scale, with_gradient(self.raw_params), self.max_norm)
         elif self.max_norm > 0:
             from .grads import clip_scale as scale_of
 
             self.grad_norm, clip_scale = scale_of(
-                [getattr(p, "grad", None) for p in self.raw_params], self.max_norm)
+                [p.grad for p in with_gradient(self.raw_params)], self.max_norm)
         self.clip_scale = clip_scale
         self.step_count += 1
         # 1. 1-D leaves: AdamW (eps 1e-8, no clip) with this optimizer's step count

@@ -69,7 +69,7 @@ class AdamW(torch.optim.Optimizer):
         """``clip_scale`` (a 0-dim f32 CUDA tensor, as ``grads.clip_scale``
         returns it) takes the place of this optimizer's own norm."""
         if clip_scale is not None:
-            check_clip_scale(clip_scale, self.param_groups[0]["max_norm"])
+            check_clip_scale(clip_scale, self._stepped(), self.param_groups[0]["max_norm"])
         loss = None
         if closure is not None:
             with torch.enable_grad():
@@ -99,9 +99,6 @@ class AdamW(torch.optim.Optimizer):
                 group["weight_decay"])
         devices = {p.device for p in params}
         if clip_scale is not None:
-            if devices != {clip_scale.device}:
-                raise ValueError("clip_scale is on the device of the parameters, got "
-                                 f"{clip_scale.device}")
             with torch.cuda.device(clip_scale.device):
                 _native.apply_pointwise(*args[:5], *args[6:], clip_scale.data_ptr(),
                                         p_dtypes=p_dt, g_dtypes=g_dt)

@@ -111,14 +111,22 @@ def _is_cuda(t) -> bool:
     return bool(getattr(t, "is_cuda", False))
 
 
-def check_clip_scale(scale, max_norm: float, in_backward: bool = False) -> None:
-    """Refuses a clip scale that a step cannot use."""
+def with_gradient(params) -> list:
+    return [p for p in params if getattr(p, "grad", None) is not None]
+
+
+def check_clip_scale(scale, stepped, max_norm: float, in_backward: bool = False) -> None:
+    """Refuses a clip scale that a step of the leaves `stepped` cannot use,
+    before it has changed anything."""
     if not _is_cuda(scale) or str(scale.dtype) != "torch.float32" or scale.numel() != 1:
         raise ValueError("clip_scale is one float32 value on a CUDA device")
     if max_norm > 0:
         raise ValueError("an optimizer with max_norm forms its own clip scale")
     if in_backward:
         raise ValueError("in_backward steps each leaf before a common norm is known")
+    for p in stepped:
+        if getattr(p, "device", None) != scale.device:
+            raise ValueError(f"clip_scale is on the device of the parameters, got {scale.device}")
 
 
 class UniversalOptimizer:
@@ -175,9 +183,6 @@ class UniversalOptimizer:
     def _call(self, p_ptrs, g_ptrs, m1_ptrs, m2_ptrs, lengths, p_dt, g_dt, step, on_device,
               device=None, clip_scale=None):
         if clip_scale is not None:
-            if not on_device or clip_scale.device != device:
-                raise ValueError("clip_scale is on the device of the parameters, got "
-                                 f"{clip_scale.device}")
             import torch
 
             with torch.cuda.device(device):
@@ -229,7 +234,9 @@ class UniversalOptimizer:
         ``grads.clip_scale`` returns it) takes the place of this optimizer's own
         norm: for a clip over more gradients than its own."""
         if clip_scale is not None:
-            check_clip_scale(clip_scale, self.max_norm, self.in_backward)
+            check_clip_scale(clip_scale,
+                             self.params if grads is not None else with_gradient(self.params),
+                             self.max_norm, self.in_backward)
         self.step_count += 1
         if self.in_backward:
             return
@@ -394,9 +401,6 @@ class _ArenaState:
                     self.grads.leaf(i).copy_(torch.as_tensor(g, device=self.device).reshape(-1))
         hp = _native.TkHParams(opt.lr, opt.beta1, opt.beta2, opt.eps, opt.weight_decay)
         if clip_scale is not None:
-            if clip_scale.device != self.device:
-                raise ValueError("clip_scale is on the device of the parameters, got "
-                                 f"{clip_scale.device}")
             with torch.cuda.device(self.device):
                 _native.check(_native.lib().tk_apply_pointwise(
                     self.leaves, self.n, _native.opt_kind(opt.algorithm), ctypes.byref(hp),
