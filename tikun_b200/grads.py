@@ -46,9 +46,11 @@ def _norm_code(norm_type) -> int:
 
 
 def _positive(max_norm) -> float:
-    if not max_norm > 0:
-        raise ValueError(f"max_norm is positive, got {max_norm!r}")
-    return float(max_norm)
+    """max_norm as the f32 number that the kernels take."""
+    value = ctypes.c_float(max_norm).value
+    if not value > 0:  # also where it is so small that it rounds to 0: no limit, there
+        raise ValueError(f"max_norm is positive as a float32, got {max_norm!r}")
+    return value
 
 
 def _dense(t: torch.Tensor) -> bool:
