@@ -177,3 +177,16 @@ def test_an_arena_takes_no_gradients_with_a_refused_scale(calls, monkeypatch):
     assert copied == [] and opt.step_count == 0
     opt.step([torch.ones(4)], clip_scale=on_device(0.5))
     assert len(copied) == 1 and opt.step_count == 1
+
+
+def test_a_closure_and_a_scale_are_refused_together(calls):
+    """The closure makes new gradients, and the scale belongs to those before."""
+    p = leaf(4)
+    opt = TorchAdamW([p])
+    ran = []
+    with pytest.raises(ValueError, match="closure"):
+        opt.step(lambda: ran.append(1), clip_scale=on_device(0.5))
+    assert not ran and not calls and opt.step_count == 0
+    opt.step(lambda: ran.append(1))
+    opt.step(clip_scale=on_device(0.5))
+    assert ran == [1] and [c[0] for c in calls] == ["step_fast_buffers_async", "apply_pointwise"]

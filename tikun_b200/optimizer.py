@@ -67,8 +67,13 @@ class AdamW(torch.optim.Optimizer):
     @torch.no_grad()
     def step(self, closure=None, clip_scale=None):
         """``clip_scale`` (a 0-dim f32 CUDA tensor, as ``grads.clip_scale``
-        returns it) takes the place of this optimizer's own norm."""
+        returns it) takes the place of this optimizer's own norm.  It belongs to
+        the gradients that are there, so a ``closure`` that makes others is
+        refused beside it."""
         if clip_scale is not None:
+            if closure is not None:
+                raise ValueError("clip_scale is of the gradients before the step; a closure would "
+                                 "make others")
             check_clip_scale(clip_scale, self._stepped(), self.param_groups[0]["max_norm"])
         loss = None
         if closure is not None:
