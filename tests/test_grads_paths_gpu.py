@@ -12,7 +12,8 @@ import pytest
 import torch
 
 from test_grads_gpu import DTYPES, IDS, NORMS, assert_norm
-from tikun_b200 import GradTable, _native
+from tikun_b200 import (GradTable, _native, accumulate_grads_, clip_grad_norm_, clip_scale,
+                        grad_norm)
 
 pytestmark = pytest.mark.gpu
 
@@ -104,3 +105,28 @@ def test_each_call_scales_by_its_own_scale():
             call("tk_clip_grad_norm", table, 2.0, norm * (0.9 - 0.07 * k), res, ws)
             assert res[1].item() < 1.0 - 0.05 * k
             assert same(out, scaled(flat, res[1]))
+
+
+@pytest.mark.parametrize("n", [1, 64, 320, 321, 400, 961, 2000])
+def test_tables_of_empty_tensors_only(n):
+    """As a rank may have whose shards are all empty: a norm of 0, nothing to scale."""
+    ts = [torch.empty(0, dtype=DTYPES[i % 3] if n == 64 else F32, device="cuda") for i in range(n)]
+    table = GradTable(ts, out=[torch.empty(0, device="cuda") for _ in ts])
+    for p in NORMS:
+        norm, each = grad_norm(ts, norm_type=p, per_tensor=True)
+        assert norm.item() == 0.0 and each.shape == (n,) and (each == 0.0).all()
+        for got in (grad_norm(ts, norm_type=p), clip_grad_norm_(ts, 1.0, norm_type=p),
+                    clip_grad_norm_(table, 1.0, norm_type=p),
+                    accumulate_grads_(table, norm_type=p)):
+            assert got.item() == 0.0
+        norm, scale = clip_scale(ts, 1.0, norm_type=p)
+        assert norm.item() == 0.0 and scale.item() == 1.0
+    accumulate_grads_(table)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        norm = clip_grad_norm_(ts, 1.0)
+        norm, each = grad_norm(ts, per_tensor=True)
+    for x in (norm, each):
+        x.fill_(7.0)
+    g.replay()
+    assert norm.item() == 0.0 and (each == 0.0).all()

@@ -843,7 +843,7 @@ int launch_fold(int norm, const double* partials, int64_t n, const NormOut& out,
     // one CTA folds 2048 partials a round; from some rounds on, a cluster does
     const int ctas = n > 8192 ? kMaxCluster : 1;
     void* args[] = {at(partials), at(n), at(out)};
-    return gr::launch((const void*)fold_kernel<decltype(k)::value>, ctas, kFoldThreads, ctas, true,
+    return gr::launch((const void*)fold_kernel<decltype(k)::value>, ctas, kFoldThreads, ctas, n > 0,
                       args, s);
   });
 }
@@ -855,7 +855,7 @@ int launch_fold_each(const GradPart& p, int norm, const double* partials, float*
       const NormOut none;
       void* args[] = {p.fold.get(), at(partials), at(each), at(all), at(n), at(out ? *out : none)};
       return gr::launch((const void*)fold_each_kernel<decltype(c)::value, decltype(k)::value>,
-                        p.n + (out ? 1 : 0), kFoldThreads, 1, true, args, s);
+                        p.n + (out ? 1 : 0), kFoldThreads, 1, n > 0, args, s);
     });
   });
 }

@@ -101,7 +101,8 @@ struct NormOut {
   float* line = nullptr;
   int n_tickets = 0;
 };
-// Both from n partials.  Enqueued right behind the launches that write them.
+// Both from n partials.  Enqueued right behind the launches that write them (of
+// none: an ordinary launch, the call's first).
 int launch_fold(int norm, const double* partials, int64_t n, const NormOut& out, cudaStream_t s);
 // Norm of each tensor of one part from its partials, into each[id]; with out,
 // the norm of n partials from `all` too.

@@ -219,6 +219,7 @@ int clip_grad_norm(const tk_grad_table& t, int norm, gr::NormOut out, void* work
   NvtxRange r("tikun/clip_grad_norm");
   if (small(t)) return gr::launch_small(t.parts[0], gr::SMALL_CLIP, norm, 0.0f, out, s);
   const size_t total = tiles_of(t);
+  if (total == 0) return gr::launch_fold(norm, nullptr, 0, out, s);  // nothing to scale
   Scratch pool;
   double* partials = nullptr;
   TK_TRY(scratch(workspace, clip_words(t), &pool, s, &partials));
