@@ -1,6 +1,7 @@
 """What the optimizers do with a clip scale of the caller's, seen from the host:
 stand-ins for CUDA tensors, and the native calls recorded in place of run."""
 import contextlib
+import ctypes
 
 import numpy as np
 import pytest
@@ -190,3 +191,12 @@ def test_a_closure_and_a_scale_are_refused_together(calls):
     opt.step(lambda: ran.append(1))
     opt.step(clip_scale=on_device(0.5))
     assert ran == [1] and [c[0] for c in calls] == ["step_fast_buffers_async", "apply_pointwise"]
+
+
+@pytest.mark.parametrize("at,text", [(0, "scale_dev is NULL"), (4097, "not aligned"), (4098, "not aligned")])
+def test_the_clipped_muon_step_refuses_an_address(at, text):
+    """A kernel would fault on it; refused before any CUDA call."""
+    hp = _native.TkMuonHParams(0.02, 0.95, 1, 5, _native.TK_NS_F16)
+    L = _native.lib()
+    assert L.tk_muon_step_clipped(None, 0, ctypes.byref(hp), at or None, None) == _native.TK_ERR_INVALID
+    assert text in L.tk_last_error().decode()

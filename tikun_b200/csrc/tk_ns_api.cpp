@@ -600,6 +600,8 @@ int tk_muon_step_clipped(const tk_muon_leaf* leaves, size_t n_leaves, const tk_m
                          const float* scale_dev, void* stream) {
   clear_error();
   if (scale_dev == nullptr) return set_error(TK_ERR_INVALID, "scale_dev is NULL");
+  if ((uintptr_t)scale_dev % 4 != 0)
+    return set_error(TK_ERR_INVALID, "scale_dev at %p is not aligned to its size", (const void*)scale_dev);
   return muon_step(leaves, n_leaves, hp, nullptr, nullptr, stream, scale_dev);
 }
 
