@@ -65,3 +65,27 @@ def test_a_scale_of_the_callers_stays_as_it_is(form):
         assert history.tolist() == [0.25, 0.5, 0.75]
         for x, y in zip(a, b):
             assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("ns_steps", [0, 5])
+@pytest.mark.parametrize("nesterov", [True, False])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_the_clipped_muon_step_at_odd_row_lengths(dtype, nesterov, ns_steps):
+    """Rows that are no multiple of four, wide, tall and by heads, with and
+    without Newton-Schulz: the bits of a step on gradients that were multiplied
+    by the scale in f32."""
+    shapes = [(33, 57), (57, 33), (1, 7), (9, 1), (3, 17, 29), (2, 70, 35), (64, 128)]
+    gen = torch.Generator().manual_seed(4)
+    ps = [torch.randn(s, generator=gen).cuda() * 0.02 for s in shapes]
+    a, b = ([torch.nn.Parameter(t.clone()) for t in ps] for _ in range(2))
+    opt_a, opt_b = (tikun_b200.MuonND(x, nesterov=nesterov, ns_steps=ns_steps) for x in (a, b))
+    for scale in (0.37, 1.0, 2.0 ** -13):
+        s = torch.tensor(scale, device="cuda")
+        for x, y in zip(a, b):
+            g = torch.randn(x.shape, generator=gen).cuda().to(dtype) * 0.1
+            x.grad_dtype = y.grad_dtype = None  # it may have another type than its parameter
+            x.grad, y.grad = g, g.float() * s
+        opt_a.step(clip_scale=s)
+        opt_b.step()
+        for x, y in zip(a, b):
+            assert torch.equal(x, y) and torch.isfinite(x).all()

@@ -130,3 +130,104 @@ def test_tables_of_empty_tensors_only(n):
         x.fill_(7.0)
     g.replay()
     assert norm.item() == 0.0 and (each == 0.0).all()
+
+
+def tile_counts(dtype):
+    """The one-cluster limit of units and one more, the limit of a fold in the scaling and
+    one more, above 52 MB of tiles that stay in L2, and a fold by a cluster."""
+    units = 32 if dtype == F32 else 16
+    return [units, units + 1, 1200, 1201, 1700, 8300]
+
+
+PATHS = [(d, t) for d in DTYPES for t in tile_counts(d)]
+PATH_IDS = [f"{dict(zip(DTYPES, IDS))[d]}-{t}" for d, t in PATHS]
+
+
+@pytest.mark.parametrize("limit", ["over", "under"])
+@pytest.mark.parametrize("target", ["in-place", "out"])
+@pytest.mark.parametrize("dtype,tiles", PATHS, ids=PATH_IDS)
+def test_clip_on_each_path(dtype, tiles, target, limit):
+    """Three calls on one table, each with fresh values, and every element compared."""
+    p = NORMS[tiles % 3]
+    flat, ts = table_of(dtype, tiles, 3)
+    out = flat if target == "in-place" else torch.empty_like(flat)
+    table = GradTable(ts, out=None if target == "in-place"
+                      else list(out.split([t.numel() for t in ts])))
+    for seed in range(3):
+        fill(flat, seed)
+        want = norm64(flat, p)
+        before = flat.clone()
+        max_norm = want * (0.3 if limit == "over" else 3.0)
+        norm = clip_grad_norm_(table, max_norm, norm_type=p)
+        assert_norm(norm, want, dtype, p)
+        scale = clip_scale_of(norm.item(), max_norm)
+        assert (scale < 1.0) == (limit == "over")
+        assert same(out, scaled(before, torch.tensor(scale, device="cuda")))
+
+
+@pytest.mark.parametrize("dtype,tiles", PATHS, ids=PATH_IDS)
+def test_norm_and_sum_on_each_path(dtype, tiles):
+    flat, ts = table_of(dtype, tiles, 4)
+    sizes = [t.numel() for t in ts]
+    acc = torch.randn(flat.numel(), device="cuda",
+                      generator=torch.Generator(device="cuda").manual_seed(5))
+    table = GradTable(ts, out=list(acc.split(sizes)))
+    for p in NORMS:
+        want = norm64(flat, p)
+        norm, each = grad_norm(table, norm_type=p, per_tensor=True)
+        assert_norm(norm, want, dtype, p)
+        assert_norm(grad_norm(table, norm_type=p), want, dtype, p)
+        for t, e in zip(ts, each.tolist()):
+            assert_norm(e, norm64(t, p), dtype, p)
+    for overwrite in (True, False):
+        # a product with a power of two is exact: one rounding of the sum on either side
+        plain = flat.float() * 0.5 + (0.0 if overwrite else acc)
+        norm = accumulate_grads_(table, alpha=0.5, overwrite=overwrite, norm_type=2.0)
+        assert torch.equal(acc, plain)
+        assert_norm(norm, norm64(acc, 2.0), F32, 2.0)
+
+
+@pytest.mark.parametrize("n", [96, 97])
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_clip_of_many_small_tensors(dtype, n):
+    """The one-cluster limit of tiles and one more."""
+    flat = torch.empty(n * 777, dtype=dtype, device="cuda")
+    fill(flat, 6)
+    before, want = flat.clone(), norm64(flat, 2.0)
+    norm = clip_grad_norm_(list(flat.split(777)), want / 3)
+    assert_norm(norm, want, dtype, 2.0)
+    assert same(flat, scaled(before, torch.tensor(clip_scale_of(norm.item(), want / 3), device="cuda")))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_captured_clips_over_a_wave_of_tickets(dtype):
+    """Two graphs, in place and out of it, with scratch of their own, replayed
+    at once on two streams with fresh values: every element scaled once."""
+    parts = []
+    for k in range(2):
+        flat, ts = table_of(dtype, 1700, 7 + k)
+        out = flat if k == 0 else torch.empty_like(flat)
+        table = GradTable(ts, out=None if k == 0 else list(out.split([t.numel() for t in ts])))
+        limit = 0.4 * norm64(flat, 2.0)
+        stream = torch.cuda.Stream()
+        clip_grad_norm_(table, 1e9)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            norm = clip_grad_norm_(table, limit)
+        parts.append((flat, out, limit, stream, graph, norm))
+    for seed in range(3):
+        before = []
+        for k, (flat, *_) in enumerate(parts):
+            fill(flat, 20 * seed + k)
+            before.append(flat.clone())
+        torch.cuda.synchronize()
+        for _, _, _, stream, graph, _ in parts:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for b, (_, out, limit, _, _, norm) in zip(before, parts):
+            assert_norm(norm, norm64(b, 2.0), dtype, 2.0)
+            scale = clip_scale_of(norm.item(), limit)
+            assert scale < 1.0
+            assert same(out, scaled(b, torch.tensor(scale, device="cuda")))
