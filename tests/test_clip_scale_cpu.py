@@ -200,3 +200,23 @@ def test_the_clipped_muon_step_refuses_an_address(at, text):
     L = _native.lib()
     assert L.tk_muon_step_clipped(None, 0, ctypes.byref(hp), at or None, None) == _native.TK_ERR_INVALID
     assert text in L.tk_last_error().decode()
+
+
+@pytest.mark.parametrize("form", ["muon", "muon_nd"])
+def test_a_step_that_forms_no_norm_shows_none(calls, monkeypatch, form):
+    """grad_norm is the last step's, so none of an earlier step's is left there."""
+    from tikun_b200 import grads, muon
+
+    formed = [(on_device(float(k)), on_device(0.5)) for k in range(3)]
+    left = iter(formed)
+    for module, name in ((grads, "clip_scale"), (muon, "scale_of")):
+        monkeypatch.setattr(module, name, lambda gs, max_norm: next(left))
+    w, b = leaf(4, 6), leaf(6)
+    opt = tikun_b200.Muon([w], [b]) if form == "muon" else tikun_b200.MuonND([w, b])
+    given = on_device(0.25)
+    for max_norm, scale, want in ((1.0, None, formed[0]), (0.0, None, (None, None)),
+                                  (1.0, None, formed[1]), (0.0, given, (None, given)),
+                                  (2.0, None, formed[2])):
+        opt.max_norm = max_norm
+        opt.step(clip_scale=scale)
+        assert opt.grad_norm is want[0] and opt.clip_scale is want[1]

@@ -63,14 +63,15 @@ class Muon(torch.optim.Optimizer):
     @torch.no_grad()
     def step(self, clip_scale=None):
         """muon.py:79-102.  ``clip_scale``: see ``MultiDimensionalMuon.step``."""
+        norm = None
         if clip_scale is not None or self.max_norm > 0:
             params = with_gradient(self.param_groups[0]["params"] +
                                    (self.adamw.params if self.adamw else []))
             if clip_scale is not None:
                 check_clip_scale(clip_scale, params, self.max_norm)
             else:
-                self.grad_norm, clip_scale = scale_of([p.grad for p in params], self.max_norm)
-        self.clip_scale = clip_scale
+                norm, clip_scale = scale_of([p.grad for p in params], self.max_norm)
+        self.grad_norm, self.clip_scale = norm, clip_scale
         self.step_count += 1
         leaves = []
         for i, p in enumerate(self.param_groups[0]["params"]):

@@ -25,7 +25,8 @@ times).
 ``max_norm`` > 0 clips all gradients, those of the Newton-Schulz leaves and of
 the AdamW leaves, by their common L2 norm, as the pointwise optimizers clip by
 theirs: the scale is folded into both updates, the gradients stay as they are,
-and ``grad_norm`` and ``clip_scale`` hold the last step's values on the device.
+and ``grad_norm`` and ``clip_scale`` hold the last step's values on the device
+(None where it formed no norm, or had no scale).
 (The reference's Muon does not clip.)
 """
 from __future__ import annotations
@@ -101,14 +102,15 @@ class MultiDimensionalMuon:
         """muon_nd.py:94-160.  ``clip_scale`` (a 0-dim f32 CUDA tensor, as
         ``grads.clip_scale`` returns it): the scale of a norm over more gradients
         than this optimizer's."""
+        norm = None
         if clip_scale is not None:
             check_clip_scale(clip_scale, with_gradient(self.raw_params), self.max_norm)
         elif self.max_norm > 0:
             from .grads import clip_scale as scale_of
 
-            self.grad_norm, clip_scale = scale_of(
-                [p.grad for p in with_gradient(self.raw_params)], self.max_norm)
-        self.clip_scale = clip_scale
+            norm, clip_scale = scale_of([p.grad for p in with_gradient(self.raw_params)],
+                                        self.max_norm)
+        self.grad_norm, self.clip_scale = norm, clip_scale
         self.step_count += 1
         # 1. 1-D leaves: AdamW (eps 1e-8, no clip) with this optimizer's step count
         if self.rank_1_params:
