@@ -52,7 +52,12 @@ constexpr int kMaxCluster = 8;  // the largest that every device setting allows
 // (small_kernel).  A clip through the Python functions, us a call among others,
 // so against in two launches: 32 whole f32 tiles 8.2 and 11.4, 48 of them 12.2
 // and 11.1; 96 tensors of 768 elements 8.2 and 11.7, 128 of them 10.3 and 11.7
-// (alone, with the wait for it, 20.4 and 19.9, 21.4 and 19.3).
+// (alone, with the wait for it, 20.4 and 19.9, 21.4 and 19.3).  The limits are
+// the clips'.  A sum with its norm would take a few more: 32 whole f32 tiles 8.2
+// and 11.6, 48 of them 10.3 and 11.7, 64 of them 12.3 and 11.6.  A norm, which
+// writes nothing, four times as many: 64 of them 8.2 and 11.6, 128 of them 10.3
+// and 11.4 (on the device, in a graph of calls, 5.5 and 3.1, 8.0 and 3.4); 256
+// tensors of 768 elements 10.3 and 11.7.
 constexpr uint32_t kSmallTiles = 96;
 constexpr uint64_t kSmallUnits = 32 * 1024;
 constexpr int kSmallThreads = 1024;
@@ -540,8 +545,9 @@ __device__ __forceinline__ void clip_tile(const GradDesc& d, uint32_t at, float 
 // ------------------------------------------------------------------ kernels
 // Tiles before `stay_from` are the first to leave L2 again: where the scaling
 // reads the last ones first, that leaves them more of it.  (GPT-2 small table,
-// f32 into f32: 226 -> 220 us for both passes; 20M elements 41 -> 38; no change
-// from 400M on.  30 to 90 MB of tiles that stay measure the same.)
+// f32 into f32: 226 -> 220 us for both passes, the scaling reads 455 of its 498
+// MB from DRAM; 20M elements 41 -> 38; no change from 400M on.  30 to 90 MB of
+// tiles that stay measure the same.)
 constexpr uint32_t kStayTiles = 1600;  // 52 MB
 
 template <int CAP, int NORM, int DT>

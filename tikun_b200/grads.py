@@ -20,7 +20,9 @@ laying out 150 tensors takes 0.1 ms of host time, a call on a table 8 us.
 
 Every call runs on torch's current stream of the gradients' device and does not
 wait for it (``error_if_nonfinite=True`` does).  A call may be captured into a
-CUDA graph.  No call is seen by autograd.
+CUDA graph.  No call is seen by autograd, and what is written in place keeps its
+version counter, as under the optimizers' steps: a tensor that a later backward
+pass still needs is not to be clipped.
 """
 from __future__ import annotations
 
@@ -269,7 +271,8 @@ def grad_norm(grads, norm_type: float = 2.0, per_tensor: bool = False,
 
 def clip_scale(grads, max_norm: float, norm_type: float = 2.0):
     """(norm, scale): the norm of ``grad_norm`` and the scale that
-    ``clip_grad_norm_`` would multiply by, both 0-dim f32 tensors on the device.
+    ``clip_grad_norm_`` would multiply by, both 0-dim f32 tensors on the device
+    that no later call or step writes.
     The optimizers' ``step(clip_scale=scale)`` folds it into their updates, so
     that several of them clip by one norm and no gradient is written."""
     code = _norm_code(norm_type)
@@ -288,9 +291,11 @@ def clip_grad_norm_(grads, max_norm: float, norm_type: float = 2.0, out=None,
     """Scales the gradients by ``max_norm / (norm + 1e-6)`` if their norm (see
     ``grad_norm``) exceeds ``max_norm``, in place or into ``out``, and returns
     the norm from before.  Each product is formed in f32 and rounded once to its
-    target's type.  The scale is the one that an optimizer with this
-    ``max_norm`` folds into its update, so clipping f32 gradients here and
-    stepping without ``max_norm`` gives the same bits.
+    target's type.  The scale is formed as an optimizer with this ``max_norm``
+    forms the one that it folds into its update, so clipping f32 gradients here
+    and stepping without ``max_norm`` gives the same bits.  Of bf16 gradients the
+    two norms, and so the scales, may differ in their last bits: the optimizer
+    adds each square in f64, ``grad_norm`` eight of them in f32 first.
 
     A norm of NaN leaves the gradients as they are (in place) or copies them
     (``out``), as the optimizers do; an infinite one makes the scale 0.
